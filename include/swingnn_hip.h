@@ -26,6 +26,11 @@ extern "C" {
 #define SWG_E_WORKSPACE (-3)   /* ws_bytes smaller than swg_workspace_bytes()             */
 #define SWG_E_NULL (-4)        /* a required pointer is NULL                              */
 
+/* element types of the operators that take more than one */
+#define SWG_F32 0
+#define SWG_BF16 1
+#define SWG_F16 2
+
 #define SWG_NOISE_EMB 512 /* noise embedding width, model/swin_gnn/swin_gnn.py:634 */
 
 /* nn.Linear as the kernels consume it: weight converted to bf16 and zero-padded along K to
@@ -452,6 +457,21 @@ int swg_adam_ema_step(const void* p_ptrs, const void* g_ptrs, const int32_t* num
                       float* ema, int64_t total, int32_t n_ema, const float* ema_decay, const float* sqnorm,
                       float max_norm, float lr, float beta1, float beta2, float eps, float weight_decay, int32_t step,
                       void* stream);
+
+/* ---- layer norm as an operator (no counterpart in the reference beyond nn.LayerNorm) ------------------------ *
+ * y = (x - mean) / sqrt(var + eps) * w + b over rows of D elements.  x, y, dy, dx: xtype (SWG_F32 / SWG_BF16 /
+ * SWG_F16), unit stride along D, row strides ld* in ELEMENTS (ldx and lddy may be 0: one row for all); no alignment
+ * beyond the element's is needed.  w, b [D] or NULL: wtype, SWG_F32 or xtype.  D <= 2^24, rows < 2^31.
+ * swg_layer_norm_fwd: mean, rstd [rows] fp32 are written for the backward pass, or both NULL.
+ * swg_layer_norm_bwd: dx, dw, db may be NULL; dw, db come in wtype, summed over the rows in fp32 in an order that
+ *   depends on (rows, D) alone.  rows == 0 writes zeros into dw, db.  ws (only with dw or db):
+ *   swg_layer_norm_bwd_workspace_bytes(rows, D, xtype), 4-byte aligned; 0 = unsupported sizes. */
+int swg_layer_norm_fwd(int64_t rows, int32_t D, const void* x, int64_t ldx, int32_t xtype, const void* w, const void* b,
+                       int32_t wtype, float eps, void* y, int64_t ldy, float* mean, float* rstd, void* stream);
+size_t swg_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t D, int32_t xtype);
+int swg_layer_norm_bwd(int64_t rows, int32_t D, const void* x, int64_t ldx, const void* dy, int64_t lddy, int32_t xtype,
+                       const void* w, int32_t wtype, const float* mean, const float* rstd, void* dx, int64_t lddx,
+                       void* dw, void* db, void* ws, size_t ws_bytes, void* stream);
 
 /* ---- post-sampling: attribute codecs of the molecule path -------------------------------- *
  * utils/attribute_code.py:14-329.  Node attributes [B,N] (int / ddpm) or [B,N,C] (one-hot / bits); adjacency

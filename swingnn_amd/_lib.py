@@ -11,6 +11,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SWG_LIB") or os.path.join(_HERE, "libswingnn_hip.so")
 
 SWG_NOISE_EMB = 512
+SWG_F32, SWG_BF16, SWG_F16 = 0, 1, 2
 ERRORS = {-1: "SWG_E_SHAPE", -2: "SWG_E_UNSUPPORTED", -3: "SWG_E_WORKSPACE", -4: "SWG_E_NULL"}
 
 _fp = C.c_void_p  # device pointers travel as void*
@@ -100,7 +101,7 @@ class SwgRefreshItem(C.Structure):
 
 
 # every symbol include/swingnn_hip.h declares: name -> (restype, argtypes)
-_i32, _sz, _f = C.c_int32, C.c_size_t, C.c_float
+_i32, _i64, _sz, _f = C.c_int32, C.c_int64, C.c_size_t, C.c_float
 SYMBOLS = {
     "swg_version": (C.c_int, []),
     "swg_workspace_bytes": (_sz, [C.POINTER(SwgNet), _i32]),
@@ -164,6 +165,10 @@ SYMBOLS = {
     "swg_grad_sqnorm": (C.c_int, [_fp, _fp, _fp, _fp, _i32, _fp, _fp]),
     "swg_adam_ema_step": (C.c_int, [_fp, _fp, _fp, _fp, _fp, _fp, _i32, _fp, _fp, _fp, C.c_int64, _i32,
                                     C.POINTER(C.c_float), _fp, _f, _f, _f, _f, _f, _f, _i32, _fp]),
+    "swg_layer_norm_fwd": (C.c_int, [_i64, _i32, _fp, _i64, _i32, _fp, _fp, _i32, _f, _fp, _i64, _fp, _fp, _fp]),
+    "swg_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "swg_layer_norm_bwd": (C.c_int, [_i64, _i32, _fp, _i64, _fp, _i64, _i32, _fp, _i32, _fp, _fp, _fp, _i64, _fp, _fp,
+                                     _fp, _sz, _fp]),
     "swg_attr_decode": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _fp, _fp, _fp, _fp, _fp, _fp]),
     "swg_attr_encode": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _fp, _fp, _fp, _fp]),
     "swg_graph_stats_workspace_bytes": (_sz, [_i32, _i32]),

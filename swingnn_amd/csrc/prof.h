@@ -40,6 +40,8 @@ enum SwgKernelId {
   KID_EXPAND_FUSED,
   KID_MLP_PROJ_192,
   KID_WATTN_RING_HD20,
+  KID_LAYER_NORM,
+  KID_ORTH,
   KID_COUNT
 };
 

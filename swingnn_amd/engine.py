@@ -32,6 +32,19 @@ def stream_ptr():
     return torch.cuda.current_stream().cuda_stream
 
 
+def call_on(device, fn, what, *args):
+    """fn(*args, current stream of `device`) with `device` current, for operators whose tensors may live on another
+    device than the current one.  The raw stream is asked for directly: a torch.cuda.Stream object costs 3 us a call
+    (8 us on autograd's thread), as much as the launch itself."""
+    idx = device.index
+    if idx == torch.cuda.current_device():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    L.check(code, what)
+
+
 _WS = {}
 _WS_PRIVATE = None   # while graphed_pass records: {(device, stream): buffer owned by the graph entry}
 

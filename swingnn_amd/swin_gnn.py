@@ -14,6 +14,7 @@ import torch.nn as nn
 
 from . import _lib as L
 from . import engine as E
+from .layer_norm import LayerNorm
 
 NOISE_EMB = L.SWG_NOISE_EMB
 
@@ -73,7 +74,7 @@ class SwinTransformerBlock(nn.Module):
                  mlp_ratio=4., qkv_bias=True, qk_scale=None, drop=0., attn_drop=0., drop_path=0.,
                  act_layer=nn.GELU, norm_layer=nn.LayerNorm):
         super().__init__()
-        if drop or drop_path or mlp_ratio != 4. or act_layer is not nn.GELU or norm_layer is not nn.LayerNorm:
+        if drop or drop_path or mlp_ratio != 4. or act_layer is not nn.GELU or norm_layer not in (nn.LayerNorm, LayerNorm):
             raise NotImplementedError("swingnn_amd supports mlp_ratio=4, GELU, LayerNorm and zero dropout / drop-path")
         if input_resolution[0] != input_resolution[1]:
             raise NotImplementedError("square token grids only (adjacency matrices)")

@@ -1,0 +1,247 @@
+"""Layer norm operator (swg_layer_norm_fwd / swg_layer_norm_bwd, swingnn_amd.layer_norm) against the formulas in float64
+on the same (already rounded) inputs.
+
+Tolerances.  u = 2^-24.  Forward, per element: mean and variance are sums over a row in float32 as trees and chains of at
+most 32 additions a lane and 12 joins (relative error <= 48 u of sum |x| / D), the division, square root and three more
+operations add a few u: |y - ref| <= 64 u (|y| + |w| max|x - mean| r + |b|) bounds all of them, plus half a step of the
+output type for its rounding.  Backward dx the same way on its three terms.  dw, db: |err| <= (rows / lanes chain + joins)
+u sum |terms|; chains here are at most 64 + 64 long: 160 u sum_rows |dy xh|, plus 64 u per term from xh: 256 u in all."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _half_step(t):
+    return 0.0 if t is F32 else torch.finfo(t).eps / 2
+
+
+def _ref(x, w, b, dy, eps):
+    """y, dx, dw, db and the magnitudes that the bounds go by, in float64."""
+    x, dy = x.double(), dy.double()
+    D = x.shape[-1]
+    w = torch.ones(D, dtype=torch.float64, device=x.device) if w is None else w.double()
+    mu = x.mean(-1, keepdim=True)
+    xc = x - mu
+    r = 1 / (xc.square().mean(-1, keepdim=True) + eps).sqrt()
+    xh = xc * r
+    y = xh * w + (0 if b is None else b.double())
+    g = dy * w
+    dx = r * (g - g.mean(-1, keepdim=True) - xh * (g * xh).mean(-1, keepdim=True))
+    # an error of mean or variance moves every element of the row: xmag bounds |x - mean| r with the cancellation in x - mean
+    xmag = (x.abs().amax(-1, keepdim=True) + mu.abs()) * r
+    ymag = w.abs() * xmag + (0 if b is None else b.double().abs())
+    gm = g.abs().amax(-1, keepdim=True)
+    dxmag = r * gm * (2 + (1 + xh.abs()) * (1 + xmag))
+    dwmag = (dy.abs() * (xh.abs() + xmag)).sum(0)
+    return y, dx, (dy * xh).sum(0), dy.sum(0), ymag, dxmag, dwmag, dy.abs().sum(0)
+
+
+def _close(got, ref, bound, what):
+    d = (got.double() - ref).abs()
+    worst = float((d - bound).detach().max()) if d.numel() else 0.0
+    assert worst <= 0, (what, worst, float(d.max()))
+
+
+def _check(x, w, b, dy, eps=1e-5):
+    import swingnn_amd as S
+    xs, ws, bs = x.detach().requires_grad_(True), None if w is None else w.detach().requires_grad_(True), \
+        None if b is None else b.detach().requires_grad_(True)
+    y = S.layer_norm(xs, ws, bs, eps)
+    leaves = [t for t in (xs, ws, bs) if t is not None]
+    grads = list(torch.autograd.grad(y, leaves, dy))
+    D = x.shape[-1]
+    x2, dy2 = x.reshape(-1, D), dy.reshape(-1, D)
+    ry, rdx, rdw, rdb, ymag, dxmag, dwmag, dbmag = _ref(x2, w, b, dy2, eps)
+    h = _half_step(x.dtype)
+    tiny = float(torch.finfo(x.dtype).tiny) * 2
+    _close(y.reshape(-1, D), ry, 64 * U * ymag + h * (ry.abs() + 64 * U * ymag) + tiny, "y")
+    _close(grads[0].reshape(-1, D), rdx, 64 * U * dxmag + h * (rdx.abs() + 64 * U * dxmag) + tiny, "dx")
+    k = 1
+    if w is not None:
+        hw = _half_step(w.dtype)
+        _close(grads[k], rdw, 256 * U * dwmag + hw * (rdw.abs() + 256 * U * dwmag) + tiny, "dw")
+        k += 1
+    if b is not None:
+        hb = _half_step(b.dtype)
+        _close(grads[k], rdb, 256 * U * dbmag + hb * (rdb.abs() + 256 * U * dbmag) + tiny, "db")
+    with torch.no_grad():
+        assert torch.equal(S.layer_norm(x, w, b, eps), y.detach())
+    again = torch.autograd.grad(S.layer_norm(xs, ws, bs, eps), leaves, dy)
+    assert all(torch.equal(p, q) for p, q in zip(grads, again)), "equal inputs, equal bits"
+
+
+def _make(shape, t, wt, bias, seed, gap=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    D = shape[-1]
+    x = (torch.randn(*shape[:-1], D + gap, device=DEV, generator=g) * 2 + 0.7).to(t)[..., :D]
+    w = None if wt is None else (1 + 0.3 * torch.randn(D, device=DEV, generator=g)).to(wt)
+    b = (0.2 * torch.randn(D, device=DEV, generator=g)).to(t if wt is None else wt) if bias else None
+    dy = torch.randn(*shape, device=DEV, generator=g).to(t)
+    return x, w, b, dy
+
+
+# one entry per register form (16-byte chunks 8 .. 4096) on both sides of its end, the looped form, widths of one and odd ones
+FP32_DIMS = [1, 2, 3, 4, 31, 32, 33, 64, 96, 97, 128, 192, 240, 256, 384, 385, 512, 768, 1000, 1024, 1025, 2047, 2048, 4096,
+             4099, 8192, 8193, 16384, 16385, 20001]
+
+
+@pytest.mark.parametrize("D", FP32_DIMS)
+def test_widths_fp32(D):
+    _check(*_make((37, D), F32, F32, True, D))
+
+
+@pytest.mark.parametrize("D", [1, 7, 8, 9, 60, 64, 65, 200, 256, 511, 1001, 2048, 4096, 8191, 16384, 16392, 32768, 32770])
+@pytest.mark.parametrize("t,wt", [(BF16, F32), (BF16, BF16), (F16, F32), (F16, F16)])
+def test_widths_half(D, t, wt):
+    _check(*_make((19, D), t, wt, True, D + 1))
+
+
+@pytest.mark.parametrize("rows", [1, 2, 31, 32, 33, 255, 4097, 40000])
+@pytest.mark.parametrize("D,t", [(60, F32), (96, F32), (257, BF16), (1536, F16)])
+def test_row_counts(rows, D, t):
+    _check(*_make((rows, D), t, F32, True, rows))
+
+
+@pytest.mark.parametrize("wt,bias", [(None, False), (None, True), (F32, False)])
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_without_weight_or_bias(wt, bias, t):
+    _check(*_make((50, 100), t, wt, bias, 3))
+
+
+@pytest.mark.parametrize("gap", [1, 3, 64])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_row_strides_and_leading_axes(gap, t):
+    _check(*_make((5, 7, 99), t, F32, True, gap, gap=gap))
+    x, w, b, dy = _make((6, 40, 33), t, F32, True, gap)
+    _check(x.transpose(0, 1), w, b, dy.transpose(0, 1))          # no uniform row stride
+    _check(x.transpose(1, 2).contiguous().transpose(1, 2), w, b, dy)  # last axis not of unit stride
+    _check(x[:, :1].expand(-1, 40, -1), w, b, dy)                # rows of stride zero
+
+
+def test_gradient_of_a_sum_and_of_parts():
+    """dy of stride zero (a sum's gradient); only some of x, weight, bias asked for."""
+    import swingnn_amd as S
+    x, w, b, dy = _make((64, 72), F32, F32, True, 9)
+    for need in ("x", "w", "b", "xw", "wb"):
+        t = {"x": x.clone(), "w": w.clone(), "b": b.clone()}
+        for k in need:
+            t[k].requires_grad_(True)
+        got = torch.autograd.grad(S.layer_norm(t["x"], t["w"], t["b"]).sum(), [t[k] for k in need])
+        _, rdx, rdw, rdb, _, dxmag, dwmag, dbmag = _ref(x, w, b, torch.ones_like(x), 1e-5)
+        want = {"x": (rdx, 64 * U * dxmag), "w": (rdw, 256 * U * dwmag), "b": (rdb, 256 * U * dbmag)}
+        for k, g in zip(need, got):
+            _close(g, want[k][0], want[k][1], k)
+
+
+def test_gradients_against_differences():
+    """Central differences of a float64 reference hold the formula; here they hold the operator's own gradient."""
+    import swingnn_amd as S
+    x, w, b, dy = _make((3, 10), F32, F32, True, 21)
+    xs, ws, bs = (t.clone().requires_grad_(True) for t in (x, w, b))
+    gx, gw, gb = torch.autograd.grad(S.layer_norm(xs, ws, bs), (xs, ws, bs), dy)
+
+    def f(x, w, b):
+        xc = x - x.mean(-1, keepdim=True)
+        return ((xc / (xc.square().mean(-1, keepdim=True) + 1e-5).sqrt() * w + b) * dy.double()).sum()
+
+    args, h = [x.double(), w.double(), b.double()], 1e-5
+    for k, g in enumerate((gx, gw, gb)):
+        flat = args[k].reshape(-1)
+        for i in range(flat.numel()):
+            keep = float(flat[i])
+            flat[i] = keep + h
+            up = float(f(*args))
+            flat[i] = keep - h
+            down = float(f(*args))
+            flat[i] = keep
+            # differences: h^2 f''' / 6 < 1e-8 at these values; the operator: its own rounding, 1e-5 of the largest gradient
+            assert abs((up - down) / (2 * h) - float(g.reshape(-1)[i])) < 1e-5 * float(g.abs().max()) + 1e-6
+
+
+def test_large_mean_and_constant_rows():
+    """A mean 4000 times the spread keeps its variance (two sums over the row, not x^2 - mean^2); equal values give the bias."""
+    import swingnn_amd as S
+    x, w, b, dy = _make((40, 384), F32, F32, True, 5)
+    _check(x * 0.5 + 4096, w, b, dy)
+    y = S.layer_norm(torch.full((4, 96), 3.0, device=DEV), w[:96], b[:96])
+    assert torch.equal(y, b[:96].expand(4, 96))
+
+
+def test_non_finite_values_stay_in_their_row():
+    import swingnn_amd as S
+    x, w, b, dy = _make((33, 96), F32, F32, True, 6)
+    clean = S.layer_norm(x, w, b)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        z = x.clone()
+        z[32, 5] = bad   # the last row: the lanes behind it work on a copy of it
+        y = S.layer_norm(z, w, b)
+        assert bool(y[32].isnan().all()) and torch.equal(y[:32], clean[:32])
+        zs = z.requires_grad_(True)
+        ws = w.clone().requires_grad_(True)
+        dx, dw = torch.autograd.grad(S.layer_norm(zs, ws, b), (zs, ws), dy)
+        assert bool(dx[:32].isfinite().all()) and bool(dw.isnan().all())
+
+
+def test_no_rows():
+    import swingnn_amd as S
+    x = torch.empty(0, 96, device=DEV, requires_grad=True)
+    w, b = torch.ones(96, device=DEV, requires_grad=True), torch.zeros(96, device=DEV, requires_grad=True)
+    y = S.layer_norm(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), torch.empty(0, 96, device=DEV))
+    assert y.shape == gx.shape == (0, 96) and not gw.any() and not gb.any()
+
+
+def test_side_stream_and_captured_graph():
+    """Forward and backward captured into a graph and replayed with new inputs, eager work between the replays."""
+    import swingnn_amd as S
+    x, w, b, dy = _make((300, 200), BF16, F32, True, 8)
+    side = torch.cuda.Stream()
+    xs, ws, bs, ds = (t.clone() for t in (x, w, b, dy))
+
+    def work():
+        a = [t.detach().requires_grad_(True) for t in (xs, ws, bs)]
+        y = S.layer_norm(*a)
+        return [y.detach()] + list(torch.autograd.grad(y, a, ds))
+
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for seed in (8, 9, 10):
+        x, w, b, dy = _make((300, 200), BF16, F32, True, seed)
+        for t, v in zip((xs, ws, bs, ds), (x, w, b, dy)):
+            t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = work()
+        assert all(torch.equal(p, q) for p, q in zip(out, want)), seed
+        if seed == 8:
+            assert all(torch.equal(p, q) for p, q in zip(first, want))
+
+
+def test_module_in_a_network():
+    """norm_layer=LayerNorm: same state dict, same forward of the network, and the norms run by themselves."""
+    import swingnn_amd as S
+    kw = dict(img_size=24, patch_size=3, in_chans=1, embed_dim=60, depths=[1, 1], num_heads=[3, 6], window_size=24, mlp_ratio=4.,
+              drop_path_rate=0., self_condition=True)
+    torch.manual_seed(0)
+    plain = S.SwinGNN(**kw).to(DEV).eval()
+    torch.manual_seed(0)
+    own = S.SwinGNN(**kw, norm_layer=S.LayerNorm).to(DEV).eval()
+    assert list(plain.state_dict()) == list(own.state_dict())
+    x, flags, lab = torch.randn(2, 24, 24, device=DEV), torch.ones(2, 24, device=DEV), torch.tensor([0.1, -0.3], device=DEV)
+    x = x + x.transpose(1, 2)
+    with torch.no_grad():
+        assert torch.equal(plain(x, flags, lab), own(x, flags, lab))
+    t = torch.randn(2, 64, 60, device=DEV, requires_grad=True)
+    y = own.norm(t)
+    assert float((y - plain.norm(t)).abs().max()) < 1e-5 and y.requires_grad
