@@ -473,6 +473,47 @@ int swg_layer_norm_bwd(int64_t rows, int32_t D, const void* x, int64_t ldx, cons
                        const void* w, int32_t wtype, const float* mean, const float* rstd, void* dx, int64_t lddx,
                        void* dw, void* db, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- orthogonalised updates (no counterpart in the reference, whose optimizers are Adam and its kin) --------- *
+ * Newton-Schulz: X0 = G / (|G|_F + eps), then `steps` (1 .. 64) times X <- a X + (b A + c A A) X with A = X X' and
+ * (a, b, c) = (3.4445, -4.7750, 2.0315).  A zero matrix gives zero; a NaN or infinity in a matrix makes it NaN.
+ * swg_orthogonalise: `count` entries (HOST array) of `batch` matrices each, any mix of shapes (rows, cols <= 2^20, 0
+ *   allowed); unit stride along a row, row strides ld_* >= cols and matrix strides bs_* in elements.  itype: SWG_F32 /
+ *   SWG_BF16 / SWG_F16; otype: SWG_BF16 / SWG_F16 (the products carry 11 bits, so there is no fp32 output).  Outputs
+ *   may not overlap inputs.  ws: swg_orthogonalise_workspace_bytes() of the same entries (0 = unsupported).
+ * swg_muon_table: writes the DEVICE table of an optimizer's matrices once (swg_muon_table_bytes(count)); its entries
+ *   name a matrix by its place in the pointer tables, so gradients and parameters may move between steps.
+ * swg_muon_ema_step, for every entry (same HOST array as the table's):
+ *   g <- g min(1, max_norm / (sqrt(*sqnorm) + 1e-6)) when sqnorm != NULL;  m <- momentum m + (1 - momentum) g;
+ *   u = nesterov ? momentum m + (1 - momentum) g : m;  p <- p (1 - lr weight_decay) - lr scale orthogonalise(u);
+ *   ema_k <- lerp(ema_k, p, 1 - ema_decay[k]) (ema_decay: HOST array).  p, g: DEVICE pointer tables, contiguous fp32;
+ *   m [total], ema [n_ema, total] at flat_off.  The matrix must not appear twice.
+ * swg_grad_sqnorm_ordered: swg_grad_sqnorm with fp64 partial sums joined in a fixed order (equal inputs, equal bits) and
+ *   without a memory clear, so it may be recorded into a graph. */
+typedef struct swg_orth_item {
+  const void* g;
+  void* out;
+  int64_t ld_g, bs_g, ld_out, bs_out;
+  int32_t rows, cols, batch, pad_;
+} swg_orth_item;
+typedef struct swg_muon_item {
+  int64_t flat_off;
+  int32_t rows, cols, index;
+  float scale;
+} swg_muon_item;
+size_t swg_orthogonalise_workspace_bytes(int32_t count, const swg_orth_item* items);
+int swg_orthogonalise(int32_t count, const swg_orth_item* items, int32_t itype, int32_t otype, int32_t steps, float eps,
+                      void* ws, size_t ws_bytes, void* stream);
+size_t swg_muon_table_bytes(int32_t count);
+int swg_muon_table(int32_t count, const swg_muon_item* items, void* table, size_t table_size, void* stream);
+size_t swg_muon_workspace_bytes(int32_t count, const swg_muon_item* items);
+int swg_muon_ema_step(int32_t count, const swg_muon_item* items, const void* table, const void* p_ptrs, const void* g_ptrs,
+                      float* m, float* ema, int64_t total, int32_t n_ema, const float* ema_decay, const float* sqnorm,
+                      float max_norm, float lr, float momentum, int32_t nesterov, float weight_decay, int32_t steps,
+                      float eps, void* ws, size_t ws_bytes, void* stream);
+size_t swg_grad_sqnorm_ordered_workspace_bytes(void);
+int swg_grad_sqnorm_ordered(const void* g_ptrs, const int32_t* numel, const int32_t* chunk_tensor, const int32_t* chunk_off,
+                            int32_t n_chunks, float* sqnorm, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- post-sampling: attribute codecs of the molecule path -------------------------------- *
  * utils/attribute_code.py:14-329.  Node attributes [B,N] (int / ddpm) or [B,N,C] (one-hot / bits); adjacency
  * attributes [B,N,N] or [B,C,N,N]; node_flags [B,N] fp32 0/1 (rows AND columns are masked for adjacency entries).

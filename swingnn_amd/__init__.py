@@ -10,11 +10,12 @@ from .swin_gnn import (SwinGNN, SwinTransformerBlock, WindowAttention, PatchMerg
 from .precond import Precond, NodeAdjPrecond
 from .edm_sampler import EDMSampler, GeneralSampler, NodeAdjEDMSampler
 from .objective import EDMObjectiveGenerator, RainbowLoss, NodeAdjEDMObjectiveGenerator, NodeAdjRainbowLoss
-from .optim import FusedAdamEMA
+from .optim import FusedAdamEMA, FusedMuonEMA
+from .orthogonalise import orthogonalise
 from .layer_norm import LayerNorm, layer_norm
 from .io import load_model, adjs_to_dataset_tensors, quantise_samples
 from . import codec, graph_stats  # noqa: F401  (post-sampling: attribute codecs, graph statistics / MMD on the device)
 
 __all__ = ["SwinGNN", "SwinTransformerBlock", "WindowAttention", "PatchMerging", "PatchBreakup", "PatchEmbed",
            "BasicLayer", "Mlp", "PositionalEmbedding", "Precond", "EDMSampler", "GeneralSampler", "EDMObjectiveGenerator", "RainbowLoss",
-           "FusedAdamEMA", "LayerNorm", "layer_norm", "NodeAdjSwinGNN", "NodeAdjPrecond", "NodeAdjEDMSampler", "NodeAdjEDMObjectiveGenerator", "NodeAdjRainbowLoss", "load_model", "adjs_to_dataset_tensors", "quantise_samples"]
+           "FusedAdamEMA", "FusedMuonEMA", "orthogonalise", "LayerNorm", "layer_norm", "NodeAdjSwinGNN", "NodeAdjPrecond", "NodeAdjEDMSampler", "NodeAdjEDMObjectiveGenerator", "NodeAdjRainbowLoss", "load_model", "adjs_to_dataset_tensors", "quantise_samples"]

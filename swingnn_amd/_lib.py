@@ -100,6 +100,16 @@ class SwgRefreshItem(C.Structure):
                 ("N", C.c_int32), ("K", C.c_int32), ("ld", C.c_int32), ("pad_", C.c_int32), ("count", C.c_int64)]
 
 
+class SwgOrthItem(C.Structure):
+    _fields_ = [("g", _fp), ("out", _fp), ("ld_g", C.c_int64), ("bs_g", C.c_int64), ("ld_out", C.c_int64),
+                ("bs_out", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32), ("batch", C.c_int32), ("pad_", C.c_int32)]
+
+
+class SwgMuonItem(C.Structure):
+    _fields_ = [("flat_off", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32), ("index", C.c_int32),
+                ("scale", C.c_float)]
+
+
 # every symbol include/swingnn_hip.h declares: name -> (restype, argtypes)
 _i32, _i64, _sz, _f = C.c_int32, C.c_int64, C.c_size_t, C.c_float
 SYMBOLS = {
@@ -169,6 +179,15 @@ SYMBOLS = {
     "swg_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i32, _i32]),
     "swg_layer_norm_bwd": (C.c_int, [_i64, _i32, _fp, _i64, _fp, _i64, _i32, _fp, _i32, _fp, _fp, _fp, _i64, _fp, _fp,
                                      _fp, _sz, _fp]),
+    "swg_orthogonalise_workspace_bytes": (_sz, [_i32, C.POINTER(SwgOrthItem)]),
+    "swg_orthogonalise": (C.c_int, [_i32, C.POINTER(SwgOrthItem), _i32, _i32, _i32, _f, _fp, _sz, _fp]),
+    "swg_muon_table_bytes": (_sz, [_i32]),
+    "swg_muon_table": (C.c_int, [_i32, C.POINTER(SwgMuonItem), _fp, _sz, _fp]),
+    "swg_muon_workspace_bytes": (_sz, [_i32, C.POINTER(SwgMuonItem)]),
+    "swg_muon_ema_step": (C.c_int, [_i32, C.POINTER(SwgMuonItem), _fp, _fp, _fp, _fp, _fp, _i64, _i32, C.POINTER(C.c_float),
+                                    _fp, _f, _f, _f, _i32, _f, _i32, _f, _fp, _sz, _fp]),
+    "swg_grad_sqnorm_ordered_workspace_bytes": (_sz, []),
+    "swg_grad_sqnorm_ordered": (C.c_int, [_fp, _fp, _fp, _fp, _i32, _fp, _fp, _sz, _fp]),
     "swg_attr_decode": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _fp, _fp, _fp, _fp, _fp, _fp]),
     "swg_attr_encode": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _fp, _fp, _fp, _fp]),
     "swg_graph_stats_workspace_bytes": (_sz, [_i32, _i32]),

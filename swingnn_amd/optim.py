@@ -20,7 +20,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from .engine import stream_ptr
+from .engine import stream_ptr, workspace
 
 
 class FusedAdamEMA(torch.optim.Optimizer):
@@ -30,18 +30,23 @@ class FusedAdamEMA(torch.optim.Optimizer):
         super().__init__(params, defaults)
         if len(self.param_groups) != 1:
             raise NotImplementedError("FusedAdamEMA: one parameter group (the reference optimises model.parameters())")
+        self._setup([p for p in self.param_groups[0]["params"]], max_norm, ema_betas, ema_inv_gamma, ema_power)
+
+    def _setup(self, params, max_norm, ema_betas, ema_inv_gamma, ema_power):
+        """Flat buffers and device tables over ``params`` in their order."""
+        name = type(self).__name__
         self.max_norm = max_norm
         self.ema_betas = tuple(sorted(float(b) for b in ema_betas))
         if len(self.ema_betas) > 8:
             raise NotImplementedError("at most 8 EMA copies")
         self.ema_inv_gamma, self.ema_power = float(ema_inv_gamma), float(ema_power)
-        self.params = [p for p in self.param_groups[0]["params"]]
+        self.params = params
         dev = self.params[0].device
         if dev.type != "cuda":
             raise RuntimeError("swingnn_amd runs on an MI355X only; there is no CPU fallback")
         for p in self.params:
             if p.dtype != torch.float32 or not p.is_contiguous() or p.device != dev:
-                raise NotImplementedError("FusedAdamEMA: contiguous fp32 parameters on one device")
+                raise NotImplementedError(f"{name}: contiguous fp32 parameters on one device")
         chunk = int(L.lib.swg_optim_chunk())
         numel, flat_off, ct, co = [], [], [], []
         off = 0
@@ -121,11 +126,11 @@ class FusedAdamEMA(torch.optim.Optimizer):
         state_dict = dict(state_dict)
         fused = state_dict.pop("fused", None)
         if fused is None:
-            raise KeyError("FusedAdamEMA.load_state_dict: no 'fused' entry (not a FusedAdamEMA checkpoint)")
+            raise KeyError(f"{type(self).__name__}.load_state_dict: no 'fused' entry (not a {type(self).__name__} checkpoint)")
         if list(fused["numel"]) != [p.numel() for p in self.params]:
-            raise ValueError("FusedAdamEMA.load_state_dict: parameter list differs from the checkpoint's")
+            raise ValueError(f"{type(self).__name__}.load_state_dict: parameter list differs from the checkpoint's")
         if [float(b) for b in fused["ema_betas"]] != list(self.ema_betas):
-            raise ValueError("FusedAdamEMA.load_state_dict: EMA betas differ from the checkpoint's")
+            raise ValueError(f"{type(self).__name__}.load_state_dict: EMA betas differ from the checkpoint's")
         super().load_state_dict(state_dict)
         self.m.copy_(fused["m"])
         self.v.copy_(fused["v"])
@@ -137,15 +142,13 @@ class FusedAdamEMA(torch.optim.Optimizer):
         """Total L2 gradient norm measured by the last step() (before clipping), as a 0-dim device tensor."""
         return self._sqnorm.sqrt().squeeze(0)
 
-    @torch.no_grad()
-    def step(self, closure=None):
-        if closure is not None:
-            raise NotImplementedError("closure")
+    def _point(self):
+        """Device tables of the gradients' and parameters' present addresses."""
         grads = []
         for p in self.params:
             g = p.grad
             if g is None:
-                raise RuntimeError("FusedAdamEMA.step: every parameter needs a gradient (the denoiser uses all of them)")
+                raise RuntimeError(f"{type(self).__name__}.step: every parameter needs a gradient (the denoiser uses all of them)")
             if g.dtype != torch.float32 or not g.is_contiguous():
                 g = p.grad = g.to(torch.float32).contiguous()
             grads.append(g)
@@ -157,6 +160,12 @@ class FusedAdamEMA(torch.optim.Optimizer):
         if pkey != self._p_key:  # parameter storage moved (model.to(), p.data = ..., load_state_dict(assign=True))
             self._p_ptrs.copy_(torch.tensor(pkey, dtype=torch.int64), non_blocking=False)
             self._p_key = pkey
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        if closure is not None:
+            raise NotImplementedError("closure")
+        self._point()
         grp = self.param_groups[0]
         st = stream_ptr()
         sq = None
@@ -185,3 +194,119 @@ class FusedAdamEMA(torch.optim.Optimizer):
         """Parameters were updated through raw pointers; bump their version counters so derived weight caches
         (engine.NetCache) rebuild: one foreach call on zero-size views (no element is touched, the counters move)."""
         torch._foreach_add_([p.view(-1)[:0] for p in self.params], 0.0)
+
+
+class FusedMuonEMA(FusedAdamEMA):
+    """Momentum with orthogonalised updates for weight matrices, Adam for the other parameters, then the clip and the EMA
+    copies of ``FusedAdamEMA`` (same flat buffers, checkpoints and EMA entries):
+
+        m <- momentum m + (1 - momentum) g;   u = momentum m + (1 - momentum) g  (m itself without ``nesterov``)
+        p <- p (1 - lr weight_decay) - lr update_rms sqrt(max(rows, cols)) orthogonalise(u)
+
+    (``swingnn_amd.orthogonalise`` with ``ns_steps`` steps).  The factor gives an update the root mean square
+    ``update_rms`` that Adam's steps have about, so both halves take one learning rate.  ``matrices``: 2-D parameters;
+    ``others``: the rest.  ``FusedMuonEMA.split(model)`` sorts a model's parameters: the weights of its ``nn.Linear``
+    layers, and everything else.  Weight decay is decoupled for the matrices and Adam's L2 term for the others.
+    Every matrix goes through the same launches: 2 + 3 ns_steps of them a step, whatever their number."""
+
+    def __init__(self, matrices, others=(), lr=1e-4, momentum=0.95, nesterov=True, ns_steps=5, weight_decay=0.0, betas=(0.9, 0.999),
+                 eps=1e-8, update_rms=0.2, max_norm=None, ema_betas=(), ema_inv_gamma=1.0, ema_power=1.0):
+        matrices, others = list(matrices), list(others)
+        if not matrices:
+            raise ValueError("FusedMuonEMA: no matrices")
+        if len({id(p) for p in matrices + others}) < len(matrices) + len(others):
+            raise ValueError("FusedMuonEMA: a parameter is given twice")
+        for p in matrices:
+            if p.dim() != 2 or p.numel() == 0:
+                raise ValueError(f"FusedMuonEMA: matrices have two axes, got shape {tuple(p.shape)}")
+        if not 1 <= int(ns_steps) <= 64:
+            raise ValueError("FusedMuonEMA: ns_steps between 1 and 64")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError("FusedMuonEMA: momentum in [0, 1)")
+        groups = [dict(params=matrices, lr=lr, momentum=momentum, nesterov=nesterov, ns_steps=int(ns_steps),
+                       weight_decay=weight_decay)]
+        if others:
+            groups.append(dict(params=others, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        torch.optim.Optimizer.__init__(self, groups, {})
+        self._setup(matrices + others, max_norm, ema_betas, ema_inv_gamma, ema_power)
+        self.n_matrices = len(matrices)
+        self.update_rms = float(update_rms)
+        dev = self.params[0].device
+        chunk = int(L.lib.swg_optim_chunk())
+        self._first_other = sum(-(-p.numel() // chunk) for p in matrices)  # chunks of the matrices come first
+        self._items = (L.SwgMuonItem * len(matrices))(*(
+            L.SwgMuonItem(o, p.shape[0], p.shape[1], i, self.update_rms * max(p.shape) ** 0.5)
+            for i, (p, o) in enumerate(zip(matrices, self._offs))))
+        self._ws_bytes = int(L.lib.swg_muon_workspace_bytes(len(matrices), self._items))
+        if self._ws_bytes == 0:
+            raise L.SwgError("swg_muon_workspace_bytes: unsupported matrix shapes")
+        nbytes = int(L.lib.swg_muon_table_bytes(len(matrices)))
+        self._table = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        self._sq_ws = torch.empty(int(L.lib.swg_grad_sqnorm_ordered_workspace_bytes()), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev):
+            L.check(L.lib.swg_muon_table(len(matrices), self._items, self._table.data_ptr(), nbytes, stream_ptr()),
+                    "swg_muon_table")
+            torch.cuda.current_stream().synchronize()  # steps may run on another stream
+
+    @staticmethod
+    def split(model):
+        """(weights of the model's nn.Linear layers, its other parameters), each parameter once."""
+        linear = {id(m.weight) for m in model.modules() if isinstance(m, torch.nn.Linear)}
+        params = list(model.parameters())
+        return [p for p in params if id(p) in linear], [p for p in params if id(p) not in linear]
+
+    def add_param_group(self, group):
+        if hasattr(self, "n_matrices"):
+            raise NotImplementedError("FusedMuonEMA: parameters are given to the constructor")
+        super().add_param_group(group)
+
+    def state_dict(self):
+        sd = super().state_dict()
+        sd["fused"]["n_matrices"] = self.n_matrices
+        return sd
+
+    def load_state_dict(self, state_dict):
+        fused = state_dict.get("fused")
+        if fused is not None and fused.get("n_matrices") != self.n_matrices:
+            raise ValueError("FusedMuonEMA.load_state_dict: another split into matrices and others than the checkpoint's")
+        super().load_state_dict(state_dict)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        if closure is not None:
+            raise NotImplementedError("closure")
+        with torch.cuda.device(self.params[0].device):
+            self._step()
+        return None
+
+    def _step(self):
+        self._point()
+        mat, st = self.param_groups[0], stream_ptr()
+        tables = (self._p_ptrs.data_ptr(), self._g_ptrs.data_ptr())
+        sq = None
+        if self.max_norm is not None:
+            sq = self._sqnorm.data_ptr()
+            L.check(L.lib.swg_grad_sqnorm_ordered(tables[1], self._numel.data_ptr(), self._ct.data_ptr(), self._co.data_ptr(),
+                                                  self.n_chunks, sq, self._sq_ws.data_ptr(), self._sq_ws.numel(), st),
+                    "swg_grad_sqnorm_ordered")
+        self.step_count += 1
+        n_ema = len(self.ema_betas)
+        dec = (C.c_float * 8)(*(self._ema_decays() + [0.0] * (8 - n_ema)))
+        clip = float(self.max_norm or 0.0)
+        ws = workspace(self.m.device, self._ws_bytes)
+        L.check(L.lib.swg_muon_ema_step(self.n_matrices, self._items, self._table.data_ptr(), *tables, self.m.data_ptr(),
+                                        self.ema.data_ptr(), self.total, n_ema, dec, sq, clip, float(mat["lr"]),
+                                        float(mat["momentum"]), int(mat["nesterov"]), float(mat["weight_decay"]),
+                                        int(mat["ns_steps"]), 1e-7, ws.data_ptr(), ws.numel(), st), "swg_muon_ema_step")
+        if len(self.param_groups) > 1:
+            grp, first = self.param_groups[1], self._first_other
+            b1, b2 = grp["betas"]
+            L.check(L.lib.swg_adam_ema_step(*tables, self._numel.data_ptr(), self._flat_off.data_ptr(),
+                                            self._ct.data_ptr() + 4 * first, self._co.data_ptr() + 4 * first,
+                                            self.n_chunks - first, self.m.data_ptr(), self.v.data_ptr(),
+                                            self.ema.data_ptr(), self.total, n_ema, dec, sq, clip, float(grp["lr"]),
+                                            float(b1), float(b2), float(grp["eps"]), float(grp["weight_decay"]),
+                                            self.step_count, st), "swg_adam_ema_step")
+        if n_ema:
+            self.ema_updates += 1
+        self._bump_versions()

@@ -57,3 +57,97 @@ def test_layer_norm_entry_points_refuse(S):
     assert w(4, 0, 0) == 0 and w(4, 8, 5) == 0
     # one partial row of 2 D sums per workgroup, at most 1024 of them
     assert w(10 ** 6, 96, 0) <= 1025 * 2 * 96 * 4 + 256
+
+
+def test_orthogonalise_refusals(S):
+    g = torch.zeros(4, 8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        S.orthogonalise(g)
+    with pytest.raises(ValueError):
+        S.orthogonalise(torch.zeros(8))
+    with pytest.raises(ValueError):
+        S.orthogonalise(torch.zeros(1, 2, 3, 4))
+    with pytest.raises(NotImplementedError):
+        S.orthogonalise(g.double())
+    with pytest.raises(NotImplementedError):
+        S.orthogonalise(g, out_dtype=torch.float32)
+    with pytest.raises(ValueError):
+        S.orthogonalise(g, steps=0)
+    with pytest.raises(ValueError):
+        S.orthogonalise(g, eps=-1.0)
+    with pytest.raises((ValueError, RuntimeError)):
+        S.orthogonalise([g, g.half()])
+    assert S.orthogonalise([]) == []
+
+
+def test_orthogonalise_entry_points_refuse(S):
+    from swingnn_amd import _lib as L
+    f, w = L.lib.swg_orthogonalise, L.lib.swg_orthogonalise_workspace_bytes
+    p = 4096
+
+    def items(rows=8, cols=8, batch=1, g=p, out=p, ld=8, ldo=8):
+        return (L.SwgOrthItem * 1)(L.SwgOrthItem(g, out, ld, 64, ldo, 64, rows, cols, batch))
+
+    big = 1 << 30
+    assert f(1, items(), 0, 1, 0, 1e-7, p, big, None) == -1
+    assert f(1, items(), 0, 1, 65, 1e-7, p, big, None) == -1
+    assert f(1, items(), 0, 1, 5, -1.0, p, big, None) == -1
+    assert f(1, items(), 0, 1, 5, float("nan"), p, big, None) == -1
+    assert f(-1, items(), 0, 1, 5, 1e-7, p, big, None) == -1
+    assert f(1, None, 0, 1, 5, 1e-7, p, big, None) == -4
+    assert f(1, items(), 3, 1, 5, 1e-7, p, big, None) == -2
+    assert f(1, items(), 0, 0, 5, 1e-7, p, big, None) == -2
+    assert f(1, items(rows=-1), 0, 1, 5, 1e-7, p, big, None) == -1
+    assert f(1, items(rows=(1 << 20) + 1), 0, 1, 5, 1e-7, p, big, None) == -1
+    assert f(1, items(ld=7), 0, 1, 5, 1e-7, p, big, None) == -1
+    assert f(1, items(ldo=7), 0, 1, 5, 1e-7, p, big, None) == -1
+    assert f(1, items(g=None), 0, 1, 5, 1e-7, p, big, None) == -4
+    assert f(1, items(), 0, 1, 5, 1e-7, None, big, None) == -4
+    assert f(1, items(), 0, 1, 5, 1e-7, p, 64, None) == -3
+    assert f(1, items(rows=0), 0, 1, 5, 1e-7, None, 0, None) == 0
+    assert f(0, None, 0, 1, 5, 1e-7, None, 0, None) == 0
+    assert w(0, items()) == 0 and w(1, None) == 0 and w(1, items(rows=-1)) == 0
+    # 6 bytes an element of X and 4 an element of A and B, padded to 32, beside the tables
+    assert w(1, items(rows=384, cols=1536)) <= 6 * 384 * 1536 + 4 * 384 * 384 + 8 * 384 + 8192
+    # sizes past 2^31 bytes keep all their terms
+    assert w(1, items(rows=40000, cols=50000)) >= 6 * 40000 * 50000 + 4 * 40000 * 40000
+
+
+def test_muon_refusals(S):
+    from swingnn_amd import _lib as L
+    P = lambda *s: torch.nn.Parameter(torch.zeros(*s))
+    a, b = P(4, 8), P(8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        S.FusedMuonEMA([a], [b])
+    with pytest.raises(ValueError):
+        S.FusedMuonEMA([], [b])
+    with pytest.raises(ValueError):
+        S.FusedMuonEMA([b])
+    with pytest.raises(ValueError):
+        S.FusedMuonEMA([a, a])
+    with pytest.raises(ValueError):
+        S.FusedMuonEMA([a], [a])
+    with pytest.raises(ValueError):
+        S.FusedMuonEMA([a], [b], ns_steps=0)
+    with pytest.raises(ValueError):
+        S.FusedMuonEMA([a], [b], momentum=1.0)
+    lin = torch.nn.Linear(3, 3)
+    tied = torch.nn.ModuleList([lin, lin, torch.nn.LayerNorm(3), torch.nn.Conv2d(1, 2, 3), torch.nn.Embedding(4, 3)])
+    mats, others = S.FusedMuonEMA.split(tied)
+    assert len(mats) == 1 and mats[0] is lin.weight and len(others) == 6
+    items = (L.SwgMuonItem * 1)(L.SwgMuonItem(0, 8, 8, 0, 1.0))
+    p, st = 4096, L.lib.swg_muon_ema_step
+    ok = [1, items, p, p, p, p, p, 64, 0, None, None, 0.0, 1e-3, 0.9, 1, 0.0, 5, 1e-7, p, 1 << 20, None]
+    for at, bad, code in ((0, 0, -1), (7, 0, -1), (8, 9, -1), (16, 0, -1), (16, 65, -1), (17, -1.0, -1), (1, None, -4), (2, None, -4), (3, None, -4),
+                          (4, None, -4), (5, None, -4), (18, None, -4), (19, 64, -3), (8, 1, -4)):
+        args = list(ok)
+        args[at] = bad
+        assert st(*args) == code, at
+    assert L.lib.swg_muon_table(0, items, p, 1 << 20, None) == -1
+    assert L.lib.swg_muon_table(1, items, p, 8, None) == -3
+    assert L.lib.swg_muon_table(1, items, None, 1 << 20, None) == -4
+    zero = (L.SwgMuonItem * 1)(L.SwgMuonItem(0, 0, 8, 0, 1.0))
+    assert L.lib.swg_muon_table(1, zero, p, 1 << 20, None) == -1
+    n = L.lib.swg_grad_sqnorm_ordered
+    assert n(None, p, p, p, 1, p, p, 8192, None) == -4 and n(p, p, p, p, 0, p, p, 8192, None) == -1
+    assert n(p, p, p, p, 1, p, p, 8, None) == -3
