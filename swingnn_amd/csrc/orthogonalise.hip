@@ -36,7 +36,7 @@ constexpr float SA = 8192.f;     // A holds A 2^13:         |A| <= 1.45  -> 11.9
 constexpr float SB = 4096.f;     // B holds B 2^12:         |B| <= 2.81  -> 11.5 k
 
 constexpr int NORM_ELEMS = 16384;  // elements per workgroup of the norm pass, at most NORM_PARTS of them per matrix
-constexpr int NORM_PARTS = 256;
+constexpr int NORM_PARTS = 1024;
 constexpr int INIT_TILE = 64;
 
 // one entry of a call: `batch` matrices of one shape (device copy in the plan, written by k_orth_table)
@@ -138,6 +138,24 @@ __device__ __forceinline__ float update_of(const Momentum& mo, float m_new, floa
   return mo.nesterov ? mo.mu * m_new + (1.f - mo.mu) * g : m_new;
 }
 
+// X lo is only ever read and written tile by tile: 16 x 32 tiles of 64 lanes x 8 elements, in the order of two
+// neighbouring accumulators (lane l holds row l & 15, columns 4 (l >> 4) .. + 3 of the first and of the second)
+__device__ __forceinline__ size_t lo_tile(int i, int j, int np) { return ((size_t)(i >> 4) * (np >> 5) + (j >> 5)) * 512; }
+__device__ __forceinline__ size_t lo_at(int i, int j, int np) {
+  return lo_tile(i, j, np) + (size_t)((((j & 15) >> 2) * 16 + (i & 15)) * 8 + ((j >> 4) & 1) * 4 + (j & 3));
+}
+// Two neighbouring accumulators as packed fp16 (columns 4 lg .. of each) <-> 8 consecutive columns per lane, starting at
+// 0, 16, 8, 24 for lane rows lg = 0 .. 3: swapping the odd lane rows of the first with the even ones of the second does
+// both directions
+__device__ __forceinline__ void swap_rows(f16x4& a, f16x4& b) {
+  uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+  const auto p = __builtin_amdgcn_permlane16_swap(x.x, y.x, false, false);
+  const auto q = __builtin_amdgcn_permlane16_swap(x.y, y.y, false, false);
+  a = __builtin_bit_cast(f16x4, make_uint2(p[0], q[0]));
+  b = __builtin_bit_cast(f16x4, make_uint2(p[1], q[1]));
+}
+__device__ __forceinline__ int swapped_col(int lg) { return 8 * (lg >> 1) + 16 * (lg & 1); }
+
 // sum of squares of a slice of a matrix into part[] (fp64: neither 1e-30 nor 1e30 leaves its range).  Momentum form: also
 // m <- mu m + (1 - mu) g, and the squares are the update's.
 template <class T, bool MOM>
@@ -149,33 +167,49 @@ __global__ __launch_bounds__(256) void k_orth_norm(const Item* __restrict__ item
   const Item& I = items[it];
   const int w = blockIdx.x - first, b = w / I.parts, k = w - b * I.parts;
   const int64_t numel = (int64_t)I.rows * I.cols;
-  const int64_t per = ((numel + I.parts - 1) / I.parts + 3) & ~(int64_t)3;
+  constexpr int N = 16 / (int)sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+  const int64_t per = ((numel + I.parts - 1) / I.parts + N - 1) / N * N;
   const int64_t lo = k * per, hi = lo + per < numel ? lo + per : numel;
   double s = 0.0;
   if constexpr (MOM) {
     const float* g = mo.g_ptrs[I.index];
     float* m = mo.m + I.flat_off;
     const float clip = clip_of(mo);
-    for (int64_t i = lo + threadIdx.x; i < hi; i += 256) {
-      const float gv = g[i] * clip, mv = new_m(mo, m[i], gv);
+    int64_t i = lo + threadIdx.x * N;
+    for (; i + N <= hi; i += 256 * N) {
+      const vec gv = *reinterpret_cast<const vec*>(g + i);
+      vec mv = *reinterpret_cast<const vec*>(m + i);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float c = gv[e] * clip;
+        mv[e] = new_m(mo, mv[e], c);
+        const double u = update_of(mo, mv[e], c);
+        s += u * u;
+      }
+      *reinterpret_cast<vec*>(m + i) = mv;
+    }
+    for (; i < hi; ++i) {  // fewer than N left: one lane's
+      const float c = g[i] * clip, mv = new_m(mo, m[i], c);
       m[i] = mv;
-      const double u = update_of(mo, mv, gv);
+      const double u = update_of(mo, mv, c);
       s += u * u;
     }
   } else {
     const T* g = (const T*)I.src + (int64_t)b * I.bs_src;
-    const int cols = I.cols;
-    if (I.ld_src == cols) {
-      for (int64_t i = lo + threadIdx.x; i < hi; i += 256) {
-        const double v = (double)(float)g[i];
-        s += v * v;
+    const bool flat = I.ld_src == I.cols;
+    // rows one after the other where they are contiguous, else row by row
+    const int64_t r_end = flat ? 1 : I.rows;
+    for (int64_t r = flat ? 0 : k; r < r_end; r += I.parts) {
+      const T* row = g + r * I.ld_src;
+      const int64_t a = flat ? lo : 0, z = flat ? hi : I.cols;
+      int64_t i = a + threadIdx.x * N;
+      for (; i + N <= z; i += 256 * N) {
+        const vec v = *reinterpret_cast<const vec*>(row + i);
+#pragma unroll
+        for (int e = 0; e < N; ++e) s += (double)(float)v[e] * (double)(float)v[e];
       }
-    } else {
-      for (int64_t i = lo + threadIdx.x; i < hi; i += 256) {
-        const int64_t r = i / cols;
-        const double v = (double)(float)g[r * I.ld_src + (i - r * cols)];
-        s += v * v;
-      }
+      for (; i < z; ++i) s += (double)(float)row[i] * (double)(float)row[i];
     }
   }
 #pragma unroll
@@ -200,7 +234,8 @@ __global__ __launch_bounds__(256) void k_orth_init(const Item* __restrict__ item
   const int b = t / (tm * tn);
   t -= b * tm * tn;
   const int i0 = (t / tn) * INIT_TILE, j0 = (t % tn) * INIT_TILE;
-  double s = (int)threadIdx.x < I.parts ? part[I.part_off + (int64_t)b * I.parts + threadIdx.x] : 0.0;
+  double s = 0.0;
+  for (int i = threadIdx.x; i < I.parts; i += 256) s += part[I.part_off + (int64_t)b * I.parts + i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -232,7 +267,7 @@ __global__ __launch_bounds__(256) void k_orth_init(const Item* __restrict__ item
     const f16 h = (f16)v;
     const size_t at = (size_t)i * I.np + j;
     B.hi(0)[at] = h;
-    B.lo[at] = (f16)(v - (float)h);
+    B.lo[lo_at(i, j, I.np)] = (f16)(v - (float)h);
   }
 }
 
@@ -250,14 +285,16 @@ __device__ __forceinline__ void wait_stage(int younger) {  // `younger` stages o
 // place of column k of B inside its 32 columns: the MFMA slots of lane group g are k = 4 g .. 4 g + 3 and 16 + 4 g ..,
 // the order in which the transposing LDS reads deliver X
 __device__ __forceinline__ int b_perm(int k) { return (k & ~31) + 8 * ((k & 15) >> 2) + 4 * ((k >> 4) & 1) + (k & 3); }
-__device__ __forceinline__ int nt_chunk(int row, int ch) { return ch ^ ((-(row >> 2)) & 3); }
+// LDS rows of 64 contraction slots (8 chunks of 16 bytes): the chunk's place in row `row`, so that the fragment reads of 16
+// rows spread over the banks.  LDS-DMA writes lanes in order, so the permutation is made on the global side.
+__device__ __forceinline__ int nt_chunk(int row, int ch) { return ch ^ (row & 7); }
 
 // A (GRAM) or B (!GRAM): T x T tile of a symmetric product P P' of one operand with contiguous contraction, T = 32 WT,
-// 4 waves of 16 WT x 16 WT.  32-deep tiles of both row panels go to LDS by LDS-DMA, NB stages.
+// 4 waves of 16 WT x 16 WT.  64-deep tiles of both row panels (whole 128-byte lines) go to LDS by LDS-DMA, NB stages.
 template <bool GRAM, int WT, int NB>
 __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ items, const int32_t* __restrict__ ends,
                                                      int count, int cur, char* __restrict__ ws) {
-  constexpr int T = 32 * WT, OP = T * 32, STAGE = 2 * OP, PER = T / 64;
+  constexpr int T = 32 * WT, OP = T * 64, STAGE = 2 * OP, PER = T / 32;
   __shared__ __attribute__((aligned(1024))) f16 sm[NB * STAGE];
   const int bid = xcd_remap(blockIdx.x, gridDim.x);
   int first;
@@ -279,20 +316,23 @@ __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ it
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wp = wave >> 1, wq = wave & 1, l15 = lane & 15, lg = lane >> 4;
   const f16 *gp[PER], *gq[PER];
+  int gc[PER];
   unsigned dst[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int j = wave + 4 * i, row = 16 * j + (lane >> 2), ch = nt_chunk(row, lane & 3) * 8;
-    gp[i] = src + (size_t)min(p0 + row, mp - 1) * ld + ch;
-    gq[i] = src + (size_t)min(q0 + row, mp - 1) * ld + ch;
+    const int j = wave + 4 * i, row = 8 * j + (lane >> 3);
+    gc[i] = nt_chunk(row, lane & 7) * 8;
+    gp[i] = src + (size_t)min(p0 + row, mp - 1) * ld;
+    gq[i] = src + (size_t)min(q0 + row, mp - 1) * ld;
     dst[i] = j * 1024;
   }
   const unsigned base = lds_addr(sm);
   auto issue = [&](int kt, int buf) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      lds_dma16(gp[i] + kt * 32, base + buf * (STAGE * 2) + dst[i]);
-      lds_dma16(gq[i] + kt * 32, base + buf * (STAGE * 2) + OP * 2 + dst[i]);
+      const int c = min(kt * 64 + gc[i], ld - 8);  // the last tile may be 32 deep: its second half is not multiplied
+      lds_dma16(gp[i] + c, base + buf * (STAGE * 2) + dst[i]);
+      lds_dma16(gq[i] + c, base + buf * (STAGE * 2) + OP * 2 + dst[i]);
     }
   };
   f32x4 acc[WT][WT];
@@ -302,12 +342,12 @@ __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ it
     for (int j = 0; j < WT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   int fp[WT], fq[WT];
 #pragma unroll
-  for (int i = 0; i < WT; ++i) {
+  for (int i = 0; i < WT; ++i) {  // rows 16 apart share their swizzle: 32 slots further is the chunk with bit 2 flipped
     const int rp = (wp * WT + i) * 16 + l15, rq = (wq * WT + i) * 16 + l15;
-    fp[i] = rp * 32 + nt_chunk(rp, lg) * 8;
-    fq[i] = OP + rq * 32 + nt_chunk(rq, lg) * 8;
+    fp[i] = rp * 64 + nt_chunk(rp, lg) * 8;
+    fq[i] = OP + rq * 64 + nt_chunk(rq, lg) * 8;
   }
-  const int nk = K / 32;
+  const int nk = (K + 63) / 64;
 #pragma unroll
   for (int st = 0; st < NB - 1; ++st)
     if (st < nk) issue(st, st);
@@ -317,16 +357,20 @@ __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ it
     __syncthreads();
     if (kt + NB - 1 < nk) issue(kt + NB - 1, buf == 0 ? NB - 1 : buf - 1);
     const f16* s = sm + buf * STAGE;
-    f16x8 vp[WT], vq[WT];
+    auto half = [&](int x) {
+      f16x8 vp[WT], vq[WT];
 #pragma unroll
-    for (int i = 0; i < WT; ++i) {
-      vp[i] = *reinterpret_cast<const f16x8*>(s + fp[i]);
-      vq[i] = *reinterpret_cast<const f16x8*>(s + fq[i]);
-    }
+      for (int i = 0; i < WT; ++i) {
+        vp[i] = *reinterpret_cast<const f16x8*>(s + (fp[i] ^ x));
+        vq[i] = *reinterpret_cast<const f16x8*>(s + (fq[i] ^ x));
+      }
 #pragma unroll
-    for (int i = 0; i < WT; ++i)
+      for (int i = 0; i < WT; ++i)
 #pragma unroll
-      for (int j = 0; j < WT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vp[i], vq[j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < WT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vp[i], vq[j], acc[i][j], 0, 0, 0);
+    };
+    half(0);
+    if (kt * 64 + 32 < K) half(32);
     buf = buf == NB - 1 ? 0 : buf + 1;
   }
 
@@ -383,12 +427,11 @@ enum { MID = 0, OUT = 1, STEP = 2 };
 
 // X' = a X + B X.  T x T tile, T = 32 WT.  B row-major (contiguous contraction), X [k][j] read through the transposing LDS
 // read.  MID writes X' as hi + lo; OUT writes O in `otype`; STEP applies the optimizer's update and the moving averages.
-// The accumulator's four registers run along j (X's rows are G's rows) or, for tall matrices in OUT / STEP, along i.
 template <int MODE, int WT, int NB>
 __global__ __launch_bounds__(256, 2) void k_orth_apply(const Item* __restrict__ items, const int32_t* __restrict__ ends,
                                                        int count, int cur, int otype, char* __restrict__ ws,
                                                        Momentum mo) {
-  constexpr int T = 32 * WT, OP = T * 32, STAGE = 2 * OP, PER = T / 64;
+  constexpr int T = 32 * WT, OP = T * 64, STAGE = 2 * OP, PER = T / 32;
   constexpr int XCH = T / 8;             // 16-byte chunks per X row in LDS
   constexpr int XROWS = 64 / XCH;        // X rows per wave transfer
   __shared__ __attribute__((aligned(1024))) f16 sm[NB * STAGE];
@@ -408,29 +451,26 @@ __global__ __launch_bounds__(256, 2) void k_orth_apply(const Item* __restrict__ 
   const int wi = wave >> 1, wj = wave & 1, l15 = lane & 15, lg = lane >> 4;
   const int q4 = l15 >> 2, p4 = l15 & 3;
   const f16 *gb[PER], *gx[PER];
+  int gc[PER], gk[PER];
   unsigned dst[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int j = wave + 4 * i, row = 16 * j + (lane >> 2);
-    gb[i] = B.B + (size_t)min(i0 + row, mp - 1) * mp + nt_chunk(row, lane & 3) * 8;
-    const int k = XROWS * j + lane / XCH;
-    const int sw = T == 128 ? 2 * (k & 7) : 2 * ((k >> 1) & 3);
-    gx[i] = X + (size_t)k * np + min(j0 + ((lane % XCH) ^ sw) * 8, np - 8);
+    const int j = wave + 4 * i, row = 8 * j + (lane >> 3);
+    gc[i] = nt_chunk(row, lane & 7) * 8;
+    gb[i] = B.B + (size_t)min(i0 + row, mp - 1) * mp;
+    gk[i] = XROWS * j + lane / XCH;
+    const int sw = T == 128 ? 2 * (gk[i] & 7) : 2 * ((gk[i] >> 1) & 3);
+    gx[i] = X + min(j0 + ((lane % XCH) ^ sw) * 8, np - 8);
     dst[i] = j * 1024;
   }
   const unsigned base = lds_addr(sm);
-  auto issue = [&](int kt, int buf) {
+  auto issue = [&](int kt, int buf) {  // the last tile may be 32 deep: its second half is not multiplied
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      lds_dma16(gb[i] + kt * 32, base + buf * (STAGE * 2) + dst[i]);
-      lds_dma16(gx[i] + (size_t)kt * 32 * np, base + buf * (STAGE * 2) + OP * 2 + dst[i]);
+      lds_dma16(gb[i] + min(kt * 64 + gc[i], mp - 8), base + buf * (STAGE * 2) + dst[i]);
+      lds_dma16(gx[i] + (size_t)min(kt * 64 + gk[i], mp - 1) * np, base + buf * (STAGE * 2) + OP * 2 + dst[i]);
     }
   };
-  f32x4 acc[WT][WT];  // [i][j]
-#pragma unroll
-  for (int i = 0; i < WT; ++i)
-#pragma unroll
-    for (int j = 0; j < WT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   int fb[WT], fx[WT];
   {
     const int r = 4 * lg + q4;  // the transposing read of k rows 4 lg .. and 16 + 4 lg ..: the swizzle is the same for both
@@ -438,136 +478,160 @@ __global__ __launch_bounds__(256, 2) void k_orth_apply(const Item* __restrict__ 
 #pragma unroll
     for (int i = 0; i < WT; ++i) {
       const int rb = (wi * WT + i) * 16 + l15;
-      fb[i] = rb * 32 + nt_chunk(rb, lg) * 8;
+      fb[i] = rb * 64 + nt_chunk(rb, lg) * 8;
       const int lc = 2 * (wj * WT + i) + (p4 >> 1);
       fx[i] = OP + r * T + (lc ^ sw) * 8 + (p4 & 1) * 4;
     }
   }
-  const bool along_i = MODE != MID && I.tall;
-  const int nk = mp / 32;
+  const int nk = (mp + 63) / 64;
 #pragma unroll
   for (int st = 0; st < NB - 1; ++st)
     if (st < nk) issue(st, st);
+  // the accumulators start as (a X + diag(B) X) 2^22, read behind the first stages' transfers; in the result a lane holds
+  // row i of X, columns j .. j + 3
+  f32x4 acc[WT][WT];  // [i][j]
+#pragma unroll
+  for (int i = 0; i < WT; ++i) {
+    const int ti = min(i0 + (wi * WT + i) * 16, mp - 16), ii = ti + l15;
+    const float e = B.dB[ii];
+#pragma unroll
+    for (int j = 0; j < WT; j += 2) {
+      const int tj = min(j0 + (wj * WT + j) * 16, np - 32);
+      const f16x8 hv = *reinterpret_cast<const f16x8*>(X + (size_t)ii * np + tj + swapped_col(lg));
+      const f16x8 lv = *reinterpret_cast<const f16x8*>(B.lo + lo_tile(ti, tj, np) + lane * 8);
+      f16x4 h[2] = {{hv[0], hv[1], hv[2], hv[3]}, {hv[4], hv[5], hv[6], hv[7]}};
+      swap_rows(h[0], h[1]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float x = (float)h[t][r];
+          acc[i][j + t][r] = (QA * (x + (float)lv[4 * t + r]) + e * x) * SB;
+        }
+    }
+  }
   int buf = 0;
   for (int kt = 0; kt < nk; ++kt) {
     wait_stage<2 * PER, NB>(min(nk - 1 - kt, NB - 2));
     __syncthreads();
     if (kt + NB - 1 < nk) issue(kt + NB - 1, buf == 0 ? NB - 1 : buf - 1);
     const f16* s = sm + buf * STAGE;
-    f16x8 vb[WT], vx[WT];
+    auto half = [&](int ks) {
+      f16x8 vb[WT], vx[WT];
 #pragma unroll
-    for (int i = 0; i < WT; ++i) {
-      vb[i] = *reinterpret_cast<const f16x8*>(s + fb[i]);
-      const f16x4 x0 = read_tr(s + fx[i]);
-      const f16x4 x1 = read_tr(s + fx[i] + 16 * T);
-      vx[i] = (f16x8){x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-    }
-    if (along_i) {
-#pragma unroll
-      for (int i = 0; i < WT; ++i)
-#pragma unroll
-        for (int j = 0; j < WT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[i], vx[j], acc[i][j], 0, 0, 0);
-    } else {
+      for (int i = 0; i < WT; ++i) {
+        vb[i] = *reinterpret_cast<const f16x8*>(s + (fb[i] ^ (32 * ks)));
+        const f16x4 x0 = read_tr(s + fx[i] + 32 * T * ks), x1 = read_tr(s + fx[i] + (32 * ks + 16) * T);
+        vx[i] = (f16x8){x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+      }
 #pragma unroll
       for (int i = 0; i < WT; ++i)
 #pragma unroll
         for (int j = 0; j < WT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vx[j], vb[i], acc[i][j], 0, 0, 0);
-    }
+    };
+    half(0);
+    if (kt * 64 + 32 < mp) half(1);
     buf = buf == NB - 1 ? 0 : buf + 1;
   }
 
-  float* p = nullptr;
-  if constexpr (MODE == STEP) p = mo.p_ptrs[I.index];
-  const float step = MODE == STEP ? mo.lr * I.scale : 0.f;
-  // four results x[r] of G's row `gr`, columns gc .. gc + 3
-  auto put = [&](int gr, int gc, const float* x) {
-    if (gr >= I.rows || gc >= I.cols) return;
-    const int have = min(4, I.cols - gc);
-    if constexpr (MODE == OUT) {
-      if (otype == SWG_BF16) {
-        bf16* d = (bf16*)I.dst + (int64_t)b * I.bs_dst + (int64_t)gr * I.ld_dst + gc;
-        if (have == 4 && ((size_t)d & 7) == 0) *reinterpret_cast<uint2*>(d) = pack_bf16x4(x[0], x[1], x[2], x[3]);
-        else
-          for (int r = 0; r < have; ++r) d[r] = (bf16)x[r];
-      } else {
-        f16* d = (f16*)I.dst + (int64_t)b * I.bs_dst + (int64_t)gr * I.ld_dst + gc;
-        if (have == 4 && ((size_t)d & 7) == 0) *reinterpret_cast<f16x4*>(d) = (f16x4){(f16)x[0], (f16)x[1], (f16)x[2], (f16)x[3]};
-        else
-          for (int r = 0; r < have; ++r) d[r] = (f16)x[r];
-      }
-    } else if constexpr (MODE == STEP) {
-      const int64_t at = (int64_t)gr * I.cols + gc;
-      float* pp = p + at;
-      float* ee = mo.ema + I.flat_off + at;
-      if (have == 4 && (((size_t)pp | (mo.n_ema ? (size_t)ee | (size_t)(mo.total * 4) : 0)) & 15) == 0) {
-        float4 v = *reinterpret_cast<float4*>(pp);
-        v.x = mo.keep * v.x - step * x[0]; v.y = mo.keep * v.y - step * x[1];
-        v.z = mo.keep * v.z - step * x[2]; v.w = mo.keep * v.w - step * x[3];
-        *reinterpret_cast<float4*>(pp) = v;
-        for (int k = 0; k < mo.n_ema; ++k) {
-          float4* e = reinterpret_cast<float4*>(ee + (int64_t)k * mo.total);
-          float4 ev = *e;
-          const float wk = mo.ema_w[k];
-          ev.x += wk * (v.x - ev.x); ev.y += wk * (v.y - ev.y); ev.z += wk * (v.z - ev.z); ev.w += wk * (v.w - ev.w);
-          *e = ev;
-        }
-      } else {
-        for (int r = 0; r < have; ++r) {
-          const float v = mo.keep * pp[r] - step * x[r];
-          pp[r] = v;
-          for (int k = 0; k < mo.n_ema; ++k) {
-            float* e = ee + (int64_t)k * mo.total + r;
-            *e += mo.ema_w[k] * (v - *e);
-          }
-        }
-      }
-    }
-  };
-  if (along_i) {
-#pragma unroll
-    for (int j = 0; j < WT; ++j) {
-      const int jj = j0 + (wj * WT + j) * 16 + l15;
-#pragma unroll
-      for (int i = 0; i < WT; ++i) {
-        const int ii = i0 + (wi * WT + i) * 16 + 4 * lg;
-        if (ii >= mp || jj >= np) continue;
-        float x[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const size_t at = (size_t)(ii + r) * np + jj;
-          const float h = (float)X[at], l = (float)B.lo[at];
-          x[r] = (QA * (h + l) + B.dB[ii + r] * h + acc[i][j][r] * (1.f / SB)) * (1.f / SX);
-        }
-        put(jj, ii, x);
-      }
-    }
-  } else {
+  if constexpr (MODE == MID) {
 #pragma unroll
     for (int i = 0; i < WT; ++i) {
-      const int ii = i0 + (wi * WT + i) * 16 + l15;
-      if (ii >= mp) continue;
-      const float e = B.dB[ii];
+      const int ti = i0 + (wi * WT + i) * 16;
 #pragma unroll
-      for (int j = 0; j < WT; ++j) {
-        const int jj = j0 + (wj * WT + j) * 16 + 4 * lg;
-        if (jj >= np) continue;
-        const size_t at = (size_t)ii * np + jj;
-        const f16x4 h4 = *reinterpret_cast<const f16x4*>(X + at), l4 = *reinterpret_cast<const f16x4*>(B.lo + at);
-        float x[4];
-        f16x4 nh, nl;
+      for (int j = 0; j < WT; j += 2) {
+        const int tj = j0 + (wj * WT + j) * 16;  // mp and np are multiples of 32: a pair of tiles is in or out
+        if (ti >= mp || tj >= np) continue;
+        f16x4 h[2];
+        f16x8 lv;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float h = (float)h4[r];
-          x[r] = QA * (h + (float)l4[r]) + e * h + acc[i][j][r] * (1.f / SB);
-          nh[r] = (f16)x[r];
-          nl[r] = (f16)(x[r] - (float)nh[r]);
-          x[r] *= 1.f / SX;
-        }
-        if constexpr (MODE == MID) {
-          *reinterpret_cast<f16x4*>(B.hi(cur ^ 1) + at) = nh;
-          *reinterpret_cast<f16x4*>(B.lo + at) = nl;
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float x = acc[i][j + t][r] * (1.f / SB);
+            h[t][r] = (f16)x;
+            lv[4 * t + r] = (f16)(x - (float)h[t][r]);
+          }
+        *reinterpret_cast<f16x8*>(B.lo + lo_tile(ti, tj, np) + lane * 8) = lv;
+        swap_rows(h[0], h[1]);
+        const f16x8 hv = {h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
+        *reinterpret_cast<f16x8*>(B.hi(cur ^ 1) + (size_t)(ti + l15) * np + tj + swapped_col(lg)) = hv;
+      }
+    }
+  }
+  if constexpr (MODE != MID) {
+    // through LDS in G's orientation, so that O (or the parameter and its averages) is touched in whole rows of the tile;
+    // 32 WT = 128: the two halves of G's rows, which two of the waves hold each, one after the other
+    constexpr int HR = T == 128 ? 64 : T, LD = T + 4;
+    static_assert(HR * LD * 4 <= NB * STAGE * 2, "the tile reuses the stages");
+    float* tile = reinterpret_cast<float*>(sm);
+    const bool tall = I.tall;
+    const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;  // G's row and column of the tile
+    float* p = nullptr;
+    if constexpr (MODE == STEP) p = mo.p_ptrs[I.index];
+    const float step = MODE == STEP ? mo.lr * I.scale : 0.f;
+    for (int half = 0; half < T / HR; ++half) {
+      __syncthreads();
+      if (T == HR || (tall ? wj : wi) == half) {
+#pragma unroll
+        for (int i = 0; i < WT; ++i)
+#pragma unroll
+          for (int j = 0; j < WT; ++j) {
+            const int li = (wi * WT + i) * 16 + l15, lj = (wj * WT + j) * 16 + 4 * lg;
+            if (tall) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) tile[(lj + r - half * HR) * LD + li] = acc[i][j][r] * (1.f / (SB * SX));
+            } else {
+              *reinterpret_cast<f32x4*>(tile + (li - half * HR) * LD + lj) = acc[i][j] * (1.f / (SB * SX));
+            }
+          }
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int k = tid; k < HR * (T / 4); k += 256) {
+        const int lr = k / (T / 4), lc = (k % (T / 4)) * 4;
+        const int gr = r0 + half * HR + lr, gc = c0 + lc;
+        if (gr >= I.rows || gc >= I.cols) continue;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(tile + lr * LD + lc);
+        const int have = min(4, I.cols - gc);
+        if constexpr (MODE == OUT) {
+          const int64_t at = (int64_t)b * I.bs_dst + (int64_t)gr * I.ld_dst + gc;
+          if (otype == SWG_BF16) {
+            bf16* d = (bf16*)I.dst + at;
+            if (have == 4 && ((size_t)d & 7) == 0) *reinterpret_cast<uint2*>(d) = pack_bf16x4(x[0], x[1], x[2], x[3]);
+            else
+              for (int r = 0; r < have; ++r) d[r] = (bf16)x[r];
+          } else {
+            f16* d = (f16*)I.dst + at;
+            const f16x4 h = {(f16)x[0], (f16)x[1], (f16)x[2], (f16)x[3]};
+            if (have == 4 && ((size_t)d & 7) == 0) *reinterpret_cast<f16x4*>(d) = h;
+            else
+              for (int r = 0; r < have; ++r) d[r] = h[r];
+          }
         } else {
-          put(ii, jj, x);
+          const int64_t at = (int64_t)gr * I.cols + gc;
+          float* pp = p + at;
+          float* ee = mo.ema + I.flat_off + at;
+          if (have == 4 && (((size_t)pp | (mo.n_ema ? (size_t)ee | (size_t)(mo.total * 4) : 0)) & 15) == 0) {
+            f32x4 v = *reinterpret_cast<f32x4*>(pp), e[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (q < mo.n_ema) e[q] = *reinterpret_cast<f32x4*>(ee + (int64_t)q * mo.total);
+            v = mo.keep * v - step * x;
+            *reinterpret_cast<f32x4*>(pp) = v;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (q < mo.n_ema) *reinterpret_cast<f32x4*>(ee + (int64_t)q * mo.total) = e[q] + mo.ema_w[q] * (v - e[q]);
+          } else {
+            for (int r = 0; r < have; ++r) {
+              const float v = mo.keep * pp[r] - step * x[r];
+              pp[r] = v;
+              for (int q = 0; q < mo.n_ema; ++q) {
+                float* e = ee + (int64_t)q * mo.total + r;
+                *e += mo.ema_w[q] * (v - *e);
+              }
+            }
+          }
         }
       }
     }
@@ -585,7 +649,14 @@ __global__ __launch_bounds__(256) void k_sqnorm_parts(const float* const* __rest
   for (int c = blockIdx.x; c < n_chunks; c += gridDim.x) {
     const int t = chunk_tensor[c], off = chunk_off[c], n = min(chunk, numel[t] - off);
     const float* g = g_ptrs[t] + off;
-    for (int i = threadIdx.x; i < n; i += 256) s += (double)g[i] * (double)g[i];
+    typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
+    const int n4 = n & ~3;
+    for (int i = 4 * threadIdx.x; i < n4; i += 1024) {
+      const vec v = *reinterpret_cast<const vec*>(g + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += (double)v[e] * (double)v[e];
+    }
+    for (int i = n4 + threadIdx.x; i < n; i += 256) s += (double)g[i] * (double)g[i];
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -608,7 +679,7 @@ constexpr int SQNORM_BLOCKS = 1024;
 // ---- host ----------------------------------------------------------------------------------------------------------
 // What a call over a list of shapes needs; the same arithmetic sizes the workspace, fills the table and sizes the grids
 struct Plan {
-  int count = 0, wt = 2;
+  int count = 0, wt_sym = 2, wt_full = 2;  // tile sides / 32
   int64_t grid[PREFIXES] = {0, 0, 0, 0, 0};
   int64_t parts = 0;
   size_t bytes = 0;                            // of X, A, B and the diagonals of all matrices
@@ -617,7 +688,7 @@ struct Plan {
 
 int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// tile side: 128 where that gives at least 1.5 workgroups a CU in the narrowest product, else 64
+// tile side of each product: 128 where that gives at least 1.5 workgroups a CU, else 64
 bool plan_item(Plan& P, int32_t rows, int32_t cols, int32_t batch, Item* I) {
   if (rows < 0 || cols < 0 || batch < 0 || rows > (1 << 20) || cols > (1 << 20)) return false;
   Item i = {};
@@ -641,13 +712,12 @@ bool plan_item(Plan& P, int32_t rows, int32_t cols, int32_t batch, Item* I) {
   if (I) *I = i;
   return true;
 }
-void plan_grids(const Item& i, int wt, int64_t* g) {
-  const int T = 32 * wt;
-  const int64_t nt = cdiv64(i.mp, T), b = i.batch;
+void plan_grids(const Item& i, int wt_sym, int wt_full, int64_t* g) {
+  const int64_t nt = cdiv64(i.mp, 32 * wt_sym), b = i.batch;
   g[P_NORM] += b * i.parts;
   g[P_INIT] += b * cdiv64(i.mp, INIT_TILE) * cdiv64(i.np, INIT_TILE);
   g[P_SYM] += b * (nt * (nt + 1) / 2);
-  g[P_FULL] += b * nt * cdiv64(i.np, T);
+  g[P_FULL] += b * cdiv64(i.mp, 32 * wt_full) * cdiv64(i.np, 32 * wt_full);
 }
 
 // plan buffer (device): Item[count], int32 ends[PREFIXES][count], then the fp64 partial sums
@@ -656,7 +726,6 @@ size_t table_bytes(int count) { return align256((size_t)count * sizeof(Item)) + 
 template <class F>
 bool make_plan(int32_t count, F shape, Plan& P) {  // shape(i, rows, cols, batch)
   if (count < 0) return false;
-  int64_t big = 0;
   for (int pass = 0; pass < 2; ++pass) {
     P.parts = 0; P.bytes = 0; P.flops = 0; P.count = 0;
     for (int k = 0; k < PREFIXES; ++k) P.grid[k] = 0;
@@ -665,11 +734,11 @@ bool make_plan(int32_t count, F shape, Plan& P) {  // shape(i, rows, cols, batch
       shape(i, r, c, b);
       Item it;
       if (!plan_item(P, r, c, b, &it)) return false;
-      plan_grids(it, pass == 0 ? 4 : P.wt, P.grid);
+      plan_grids(it, pass == 0 ? 4 : P.wt_sym, pass == 0 ? 4 : P.wt_full, P.grid);
     }
     if (pass == 0) {
-      big = P.grid[P_SYM];
-      P.wt = big >= 384 ? 4 : 2;
+      P.wt_sym = P.grid[P_SYM] >= 384 ? 4 : 2;
+      P.wt_full = P.grid[P_FULL] >= 384 ? 4 : 2;
     }
   }
   for (int k = 0; k < PREFIXES; ++k)
@@ -688,7 +757,7 @@ int write_table(int32_t count, const Plan& P, F fill, void* table, hipStream_t s
     const int n = count - first < TABLE_BATCH ? count - first : TABLE_BATCH;
     for (int k = 0; k < n; ++k) {
       fill(first + k, run, eb.e[k].item);
-      plan_grids(eb.e[k].item, P.wt, g);
+      plan_grids(eb.e[k].item, P.wt_sym, P.wt_full, g);
       for (int q = 0; q < PREFIXES; ++q) eb.e[k].end[q] = (int32_t)g[q];
     }
     hipLaunchKernelGGL(k_orth_table, dim3(1), dim3(64), 0, s, eb, first, n, count, items, ends);
@@ -717,26 +786,31 @@ Ptrs ptrs_of(int count, const Plan& P, const void* table, void* ws) {
 }
 
 template <int MODE, int WT, int NB>
-int run_steps(const Plan& P, const Ptrs& p, int steps, int otype, const Momentum& mo, hipStream_t s) {
-  const dim3 gs((unsigned)P.grid[P_SYM]), gf((unsigned)P.grid[P_FULL]);
-  int cur = 0;
-  for (int k = 0; k < steps; ++k) {
-    hipLaunchKernelGGL((k_orth_sym<true, WT, NB>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
-    hipLaunchKernelGGL((k_orth_sym<false, WT, NB>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
-    if (k + 1 < steps)
-      hipLaunchKernelGGL((k_orth_apply<MID, WT, NB>), gf, dim3(256), 0, s, p.items, p.end(P_FULL), p.count, cur, otype,
-                         p.ws, mo);
-    else
-      hipLaunchKernelGGL((k_orth_apply<MODE, WT, NB>), gf, dim3(256), 0, s, p.items, p.end(P_FULL), p.count, cur, otype,
-                         p.ws, mo);
-    SWG_LAUNCH_CHECK();
-    cur ^= 1;
-  }
-  return 0;
+void apply(const Plan& P, const Ptrs& p, int cur, int otype, const Momentum& mo, hipStream_t s) {
+  hipLaunchKernelGGL((k_orth_apply<MODE, WT, NB>), dim3((unsigned)P.grid[P_FULL]), dim3(256), 0, s, p.items, p.end(P_FULL),
+                     p.count, cur, otype, p.ws, mo);
 }
 template <int MODE>
 int run_steps(const Plan& P, const Ptrs& p, int steps, int otype, const Momentum& mo, hipStream_t s) {
-  return P.wt == 4 ? run_steps<MODE, 4, 3>(P, p, steps, otype, mo, s) : run_steps<MODE, 2, 4>(P, p, steps, otype, mo, s);
+  const dim3 gs((unsigned)P.grid[P_SYM]);
+  for (int k = 0, cur = 0; k < steps; ++k, cur ^= 1) {
+    if (P.wt_sym == 4) {
+      hipLaunchKernelGGL((k_orth_sym<true, 4, 2>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
+      hipLaunchKernelGGL((k_orth_sym<false, 4, 2>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
+    } else {
+      hipLaunchKernelGGL((k_orth_sym<true, 2, 3>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
+      hipLaunchKernelGGL((k_orth_sym<false, 2, 3>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
+    }
+    if (k + 1 < steps) {
+      if (P.wt_full == 4) apply<MID, 4, 2>(P, p, cur, otype, mo, s);
+      else apply<MID, 2, 3>(P, p, cur, otype, mo, s);
+    } else {
+      if (P.wt_full == 4) apply<MODE, 4, 2>(P, p, cur, otype, mo, s);
+      else apply<MODE, 2, 3>(P, p, cur, otype, mo, s);
+    }
+    SWG_LAUNCH_CHECK();
+  }
+  return 0;
 }
 
 template <class T, bool MOM>
