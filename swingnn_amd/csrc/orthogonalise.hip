@@ -52,10 +52,11 @@ struct Item {
   int32_t parts;     // workgroups of the norm pass per matrix
   int64_t part_off;  // first fp64 partial of the item
   float scale;       // momentum form: update = lr scale O
-  int32_t pad_;
+  int32_t small;     // all steps in one workgroup
 };
-constexpr int PREFIXES = 5;  // running workgroup counts: norm, init, symmetric products, X product, (reserved)
-enum { P_NORM = 0, P_INIT, P_SYM, P_FULL, P_SPARE };
+// running workgroup counts: norm, init, symmetric products, X product, whole small matrices, last X product
+constexpr int PREFIXES = 6;
+enum { P_NORM = 0, P_INIT, P_SYM, P_FULL, P_SMALL, P_LAST };
 struct Entry {
   Item item;
   int32_t end[PREFIXES];  // running totals including this item
@@ -141,9 +142,6 @@ __device__ __forceinline__ float update_of(const Momentum& mo, float m_new, floa
 // X lo is only ever read and written tile by tile: 16 x 32 tiles of 64 lanes x 8 elements, in the order of two
 // neighbouring accumulators (lane l holds row l & 15, columns 4 (l >> 4) .. + 3 of the first and of the second)
 __device__ __forceinline__ size_t lo_tile(int i, int j, int np) { return ((size_t)(i >> 4) * (np >> 5) + (j >> 5)) * 512; }
-__device__ __forceinline__ size_t lo_at(int i, int j, int np) {
-  return lo_tile(i, j, np) + (size_t)((((j & 15) >> 2) * 16 + (i & 15)) * 8 + ((j >> 4) & 1) * 4 + (j & 3));
-}
 // Two neighbouring accumulators as packed fp16 (columns 4 lg .. of each) <-> 8 consecutive columns per lane, starting at
 // 0, 16, 8, 24 for lane rows lg = 0 .. 3: swapping the odd lane rows of the first with the even ones of the second does
 // both directions
@@ -219,7 +217,8 @@ __global__ __launch_bounds__(256) void k_orth_norm(const Item* __restrict__ item
   if (threadIdx.x == 0) part[I.part_off + w] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// X0 = G / (|G|_F + eps) as hi + lo, transposed where the matrix is tall, zero in the padding.  One 64 x 64 tile of X.
+// X0 = G / (|G|_F + eps) as hi + lo, transposed where the matrix is tall, zero in the padding.  One 64 x 64 tile of X: a wave
+// writes 16 x 32 pairs of accumulator tiles as the products do.  Tall matrices come through LDS.
 template <class T, bool MOM>
 __global__ __launch_bounds__(256) void k_orth_init(const Item* __restrict__ items, const int32_t* __restrict__ ends,
                                                    int count, const double* __restrict__ part, double eps,
@@ -234,40 +233,87 @@ __global__ __launch_bounds__(256) void k_orth_init(const Item* __restrict__ item
   const int b = t / (tm * tn);
   t -= b * tm * tn;
   const int i0 = (t / tn) * INIT_TILE, j0 = (t % tn) * INIT_TILE;
-  double s = 0.0;
-  for (int i = threadIdx.x; i < I.parts; i += 256) s += part[I.part_off + (int64_t)b * I.parts + i];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  const double inv = (double)SX / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + eps);
   const Bufs B = bufs_of(I, ws, b);
   const T* g = MOM ? nullptr : (const T*)I.src + (int64_t)b * I.bs_src;
   const float* gm = MOM ? mo.g_ptrs[I.index] : nullptr;
   const float* m = MOM ? mo.m + I.flat_off : nullptr;
   const float clip = MOM ? clip_of(mo) : 1.f;
   const int64_t ld = MOM ? I.cols : I.ld_src;
-  auto value = [&](int r, int c) -> float {  // row and column of G
-    if (r >= I.rows || c >= I.cols) return 0.f;
+  // columns c .. c + 3 of G's row r, zero behind its edges
+  auto four = [&](int r, int c, float (&v)[4]) {
+    typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    typedef float fvec __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = 0.f;
+    if (r >= I.rows || c >= I.cols) return;
     const int64_t at = (int64_t)r * ld + c;
-    float v;
-    if constexpr (MOM) v = update_of(mo, m[at], gm[at] * clip);
-    else v = (float)g[at];
-    return (float)((double)v * inv);
+    if (c + 3 < I.cols) {
+      if constexpr (MOM) {
+        const fvec a = *reinterpret_cast<const fvec*>(gm + at), o = *reinterpret_cast<const fvec*>(m + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = update_of(mo, o[e], a[e] * clip);
+      } else {
+        const vec a = *reinterpret_cast<const vec*>(g + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)a[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < I.cols) v[e] = MOM ? update_of(mo, m[at + e], gm[at + e] * clip) : (float)g[at + e];
+    }
   };
-  if (I.tall) {
-    for (int k = threadIdx.x; k < INIT_TILE * INIT_TILE; k += 256)
-      tile[k & 63][k >> 6] = value(j0 + (k >> 6), i0 + (k & 63));
-    __syncthreads();
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, lg = lane >> 4;
+  const bool tall = I.tall;
+  const int ti = i0 + wave * 16;  // this wave's 16 rows of the tile, two pairs of column tiles
+  float v[2][2][4];
+  if (tall) {
+    float u[4][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) four(j0 + k * 16 + (tid >> 4), i0 + (tid & 15) * 4, u[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tile[(tid & 15) * 4 + e][k * 16 + (tid >> 4)] = u[k][e];
+  } else {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) four(ti + l15, j0 + q * 32 + h * 16 + 4 * lg, v[q][h]);
   }
-  for (int k = threadIdx.x; k < INIT_TILE * INIT_TILE; k += 256) {
-    const int i = i0 + (k >> 6), j = j0 + (k & 63);
-    if (i >= I.mp || j >= I.np) continue;
-    const float v = I.tall ? tile[k >> 6][k & 63] : value(i, j);
-    const f16 h = (f16)v;
-    const size_t at = (size_t)i * I.np + j;
-    B.hi(0)[at] = h;
-    B.lo[lo_at(i, j, I.np)] = (f16)(v - (float)h);
+  double s = 0.0;
+  for (int i = tid; i < I.parts; i += 256) s += part[I.part_off + (int64_t)b * I.parts + i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (lane == 0) red[wave] = s;
+  __syncthreads();
+  const double inv = (double)SX / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + eps);
+  if (tall) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[q][h][e] = tile[wave * 16 + l15][q * 32 + h * 16 + 4 * lg + e];
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int tj = j0 + q * 32;
+    if (ti >= I.mp || tj >= I.np) continue;
+    f16x4 h[2];
+    f16x8 lv;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = (float)((double)v[q][k][e] * inv);
+        h[k][e] = (f16)x;
+        lv[4 * k + e] = (f16)(x - (float)h[k][e]);
+      }
+    *reinterpret_cast<f16x8*>(B.lo + lo_tile(ti, tj, I.np) + lane * 8) = lv;
+    swap_rows(h[0], h[1]);
+    const f16x8 hv = {h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
+    *reinterpret_cast<f16x8*>(B.hi(0) + (size_t)(ti + l15) * I.np + tj + swapped_col(lg)) = hv;
   }
 }
 
@@ -291,6 +337,7 @@ __device__ __forceinline__ int nt_chunk(int row, int ch) { return ch ^ (row & 7)
 
 // A (GRAM) or B (!GRAM): T x T tile of a symmetric product P P' of one operand with contiguous contraction, T = 32 WT,
 // 4 waves of 16 WT x 16 WT.  64-deep tiles of both row panels (whole 128-byte lines) go to LDS by LDS-DMA, NB stages.
+constexpr int SYM_TILE = 64;
 template <bool GRAM, int WT, int NB>
 __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ items, const int32_t* __restrict__ ends,
                                                      int count, int cur, char* __restrict__ ws) {
@@ -445,7 +492,8 @@ __global__ __launch_bounds__(256, 2) void k_orth_apply(const Item* __restrict__ 
   t -= b * ntm * ntn;
   const int i0 = (t % ntm) * T, j0 = (t / ntm) * T;
   const Bufs B = bufs_of(I, ws, b);
-  const f16* X = B.hi(cur);
+  const bool done = MODE == STEP && I.small;  // its steps are made: only the results are left to apply
+  const f16* X = B.hi(done ? 0 : cur);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wi = wave >> 1, wj = wave & 1, l15 = lane & 15, lg = lane >> 4;
@@ -483,7 +531,7 @@ __global__ __launch_bounds__(256, 2) void k_orth_apply(const Item* __restrict__ 
       fx[i] = OP + r * T + (lc ^ sw) * 8 + (p4 & 1) * 4;
     }
   }
-  const int nk = (mp + 63) / 64;
+  const int nk = done ? 0 : (mp + 63) / 64;
 #pragma unroll
   for (int st = 0; st < NB - 1; ++st)
     if (st < nk) issue(st, st);
@@ -493,7 +541,7 @@ __global__ __launch_bounds__(256, 2) void k_orth_apply(const Item* __restrict__ 
 #pragma unroll
   for (int i = 0; i < WT; ++i) {
     const int ti = min(i0 + (wi * WT + i) * 16, mp - 16), ii = ti + l15;
-    const float e = B.dB[ii];
+    const float a = done ? 1.f : QA, e = done ? 0.f : B.dB[ii];
 #pragma unroll
     for (int j = 0; j < WT; j += 2) {
       const int tj = min(j0 + (wj * WT + j) * 16, np - 32);
@@ -506,7 +554,7 @@ __global__ __launch_bounds__(256, 2) void k_orth_apply(const Item* __restrict__ 
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float x = (float)h[t][r];
-          acc[i][j + t][r] = (QA * (x + (float)lv[4 * t + r]) + e * x) * SB;
+          acc[i][j + t][r] = (a * (x + (float)lv[4 * t + r]) + e * x) * SB;
         }
     }
   }
@@ -587,28 +635,39 @@ __global__ __launch_bounds__(256, 2) void k_orth_apply(const Item* __restrict__ 
           }
       }
       __syncthreads();
-#pragma unroll 1
-      for (int k = tid; k < HR * (T / 4); k += 256) {
-        const int lr = k / (T / 4), lc = (k % (T / 4)) * 4;
-        const int gr = r0 + half * HR + lr, gc = c0 + lc;
-        if (gr >= I.rows || gc >= I.cols) continue;
-        const f32x4 x = *reinterpret_cast<const f32x4*>(tile + lr * LD + lc);
-        const int have = min(4, I.cols - gc);
-        if constexpr (MODE == OUT) {
-          const int64_t at = (int64_t)b * I.bs_dst + (int64_t)gr * I.ld_dst + gc;
+      if constexpr (MODE == OUT) {
+#pragma unroll 2
+        for (int k = tid; k < HR * (T / 8); k += 256) {
+          const int lr = k / (T / 8), lc = (k % (T / 8)) * 8;
+          const int gr = r0 + half * HR + lr, gc = c0 + lc;
+          if (gr >= I.rows || gc >= I.cols) continue;
+          const f32x4 x0 = *reinterpret_cast<const f32x4*>(tile + lr * LD + lc), x1 = *reinterpret_cast<const f32x4*>(tile + lr * LD + lc + 4);
+          uint4 u;  // eight results of either type
           if (otype == SWG_BF16) {
-            bf16* d = (bf16*)I.dst + at;
-            if (have == 4 && ((size_t)d & 7) == 0) *reinterpret_cast<uint2*>(d) = pack_bf16x4(x[0], x[1], x[2], x[3]);
-            else
-              for (int r = 0; r < have; ++r) d[r] = (bf16)x[r];
+            const uint2 a = pack_bf16x4(x0[0], x0[1], x0[2], x0[3]), c = pack_bf16x4(x1[0], x1[1], x1[2], x1[3]);
+            u = make_uint4(a.x, a.y, c.x, c.y);
           } else {
-            f16* d = (f16*)I.dst + at;
-            const f16x4 h = {(f16)x[0], (f16)x[1], (f16)x[2], (f16)x[3]};
-            if (have == 4 && ((size_t)d & 7) == 0) *reinterpret_cast<f16x4*>(d) = h;
-            else
-              for (int r = 0; r < have; ++r) d[r] = h[r];
+            u = __builtin_bit_cast(uint4, (f16x8){(f16)x0[0], (f16)x0[1], (f16)x0[2], (f16)x0[3], (f16)x1[0], (f16)x1[1],
+                                                  (f16)x1[2], (f16)x1[3]});
           }
-        } else {
+          uint16_t* d = (uint16_t*)I.dst + (int64_t)b * I.bs_dst + (int64_t)gr * I.ld_dst + gc;
+          typedef uint16_t vec __attribute__((ext_vector_type(8), aligned(2)));
+          const vec w = __builtin_bit_cast(vec, u);
+          if (gc + 7 < I.cols) *reinterpret_cast<vec*>(d) = w;
+          else {
+#pragma unroll
+            for (int r = 0; r < 7; ++r)
+              if (gc + r < I.cols) d[r] = w[r];
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int k = tid; k < HR * (T / 4); k += 256) {
+          const int lr = k / (T / 4), lc = (k % (T / 4)) * 4;
+          const int gr = r0 + half * HR + lr, gc = c0 + lc;
+          if (gr >= I.rows || gc >= I.cols) continue;
+          const f32x4 x = *reinterpret_cast<const f32x4*>(tile + lr * LD + lc);
+          const int have = min(4, I.cols - gc);
           const int64_t at = (int64_t)gr * I.cols + gc;
           float* pp = p + at;
           float* ee = mo.ema + I.flat_off + at;
@@ -635,6 +694,393 @@ __global__ __launch_bounds__(256, 2) void k_orth_apply(const Item* __restrict__ 
         }
       }
     }
+  }
+}
+
+// ---- small matrices: all steps in one workgroup ---------------------------------------------------------------------
+// X stays in the accumulators of 8 waves for the whole call (fp32: no lo), its fp16 form in LDS; wave w owns the columns
+// of tiles w njw .. of 16.  Per step: A by 32 x 32 blocks (K split over waves where there are few), B in A's place, then
+// every wave multiplies its own columns and writes their fp16 form back (no other wave reads them before the barrier).
+// Against 2 + 3 steps launches this saves their latencies, which are all that such a matrix costs there.  Measured, five
+// steps, this form / the launches: 32 x 32 21 / 49 us, 96 x 96 32 / 65, 60 x 240 30 / 66, 96 x 384 47 / 77, 128 x 384 77 / 80,
+// 32 x 2048 79 / 122, 512 of 96 x 96 66 / 180; a fourth column tile a wave at 128 rows spills (120 x 512: 112 / 86).
+struct SmallGeom {
+  int mr, ldx, lda;       // rows of X kept in LDS, row strides (elements) of X and A
+  int off_a, off_d, off_red, bytes;
+};
+constexpr int SMALL_LDS = 163840, SMALL_WAVES = 8;
+// number of waves that share the contraction of a 32 x 32 block of A
+__host__ __device__ inline int small_split(int mp) { return mp == 32 ? 4 : mp == 64 ? 2 : 1; }
+__host__ __device__ inline SmallGeom small_geom(int m, int mp, int np) {
+  SmallGeom g;
+  g.ldx = np + 8;  // 16 bytes more than a multiple of the banks: the 16 rows of a fragment read spread over them
+  g.lda = mp + 8;
+  const int a = mp * g.lda * 2, nb = mp / 32, blocks = nb * (nb + 1) / 2;
+  const int rest = a + 2 * mp * 4 + blocks * (small_split(mp) - 1) * 4096 + 64;
+  g.mr = mp;
+  // X's rows behind m are only ever multiplied by zeros of B or left out: they may lie in A's place, which is finite
+  if (mp * g.ldx * 2 + rest > SMALL_LDS && (mp - ((m + 7) & ~7)) * g.ldx * 2 <= a) g.mr = (m + 7) & ~7;
+  g.off_a = g.mr * g.ldx * 2;
+  g.off_d = g.off_a + a;
+  g.off_red = g.off_d + 2 * mp * 4;
+  g.bytes = g.off_a + rest;
+  return g;
+}
+__host__ __device__ inline int small_nj(int mt) { return mt == 2 ? 16 : mt == 4 ? 8 : mt == 6 ? 5 : 3; }  // column tiles a wave holds
+inline bool is_small(int m, int mp, int np) {
+  return mp <= 128 && (np / 16 + SMALL_WAVES - 1) / SMALL_WAVES <= small_nj(mp / 16) && small_geom(m, mp, np).bytes <= SMALL_LDS;
+}
+
+// 0 that the compiler cannot see through: addresses formed with it are not kept in registers over the steps, where the
+// accumulators need the room
+__device__ __forceinline__ int opaque0() {
+  int o;
+  asm volatile("s_mov_b32 %0, 0" : "=s"(o));
+  return o;
+}
+
+// X's row i, columns j .. j + 3, in a matrix of G's layout: a vector of four, or four rows where the matrix is tall
+template <class T>
+__device__ __forceinline__ f32x4 load4(const T* g, const Item& I, int64_t ld, bool tall, int i, int j) {
+  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (i >= I.m) return v;
+  if (!tall && j + 3 < I.n) {
+    const vec t = *reinterpret_cast<const vec*>(g + (int64_t)i * ld + j);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = (float)t[r];
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (j + r < I.n) v[r] = (float)g[tall ? (int64_t)(j + r) * ld + i : (int64_t)i * ld + j + r];
+  }
+  return v;
+}
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));  // four rounded results of either type
+template <class T, class V>
+__device__ __forceinline__ void store4(T* g, const Item& I, int64_t ld, bool tall, int i, int j, V v) {
+  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (i >= I.m) return;
+  if (!tall && j + 3 < I.n) {
+    vec t;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) t[r] = (T)v[r];
+    *reinterpret_cast<vec*>(g + (int64_t)i * ld + j) = t;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (j + r < I.n) g[tall ? (int64_t)(j + r) * ld + i : (int64_t)i * ld + j + r] = (T)v[r];
+  }
+}
+
+template <class T, bool MOM, int MT, int NJ>
+__device__ __forceinline__ void small_body(const Item& I, int b, int steps, double eps, int otype, char* ws,
+                                           char* lds) {
+  const int m = I.m, mp = I.mp, np = I.np, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int l15 = lane & 15, lg = lane >> 4, q4 = l15 >> 2, p4 = l15 & 3;
+  const SmallGeom G = small_geom(m, mp, np);
+  f16* X = (f16*)lds;
+  f16* A = (f16*)(lds + G.off_a);
+  float *dA = (float*)(lds + G.off_d), *dB = dA + mp;
+  double* red = (double*)(lds + G.off_red);
+  float* scr = (float*)(lds + G.off_red);
+  const int ntj = np / 16, njw = (ntj + SMALL_WAVES - 1) / SMALL_WAVES, jt0 = wave * njw;
+  const bool tall = I.tall;
+  constexpr int CH = 2;
+
+  f32x4 x[MT][NJ];
+  const Bufs W = MOM ? bufs_of(I, ws, b) : Bufs{};
+  float inv = 1.f;
+  int inv_exp = 0;  // 1 / (|G| + eps) as inv 2^inv_exp: it may lie outside fp32's range
+  if constexpr (MOM) {  // X0 is there (the norm and the momentum take more bandwidth than one workgroup has)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int jj = min(jt0 + j, ntj - 1) * 16;
+        const f16x4 h = *reinterpret_cast<const f16x4*>(W.hi(0) + (size_t)(i * 16 + l15) * np + jj + 4 * lg);
+        const f16x4 l = *reinterpret_cast<const f16x4*>(W.lo + lo_tile(i * 16, jj, np) + lane * 8 + (jj >> 4 & 1) * 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[i][j][r] = (float)h[r] + (float)l[r];
+      }
+    }
+  } else {
+    double s = 0.0;
+    const T* g = (const T*)I.src + (int64_t)b * I.bs_src;
+    // up to CH tiles in flight at a time
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j0 = 0; j0 < NJ; j0 += CH) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int ii = i * 16 + l15 + opaque0(), jb = (jt0 + j0) * 16 + 4 * lg, have = min(njw, ntj - jt0) - j0;
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+          if (j0 + j >= NJ) continue;
+          x[i][j0 + j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+          if (j < have) x[i][j0 + j] = load4(g, I, I.ld_src, tall, ii, jb + 16 * j);
+        }
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+          if (j0 + j >= NJ) continue;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s += (double)x[i][j0 + j][r] * (double)x[i][j0 + j][r];
+        }
+      }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) red[wave] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int w = 0; w < SMALL_WAVES; ++w) s += red[w];
+    inv = (float)frexp((double)SX / (sqrt(s) + eps), &inv_exp);
+  }
+  // this wave's columns of X as fp16: two neighbouring tiles would be 16 bytes a lane, one is 8
+  auto put_hi = [&]() {
+    const int o = opaque0();
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int ii = i * 16 + l15 + o;
+        __builtin_amdgcn_sched_barrier(0);
+        if (j >= njw || jt0 + j >= ntj || ii >= G.mr) continue;
+        *reinterpret_cast<f16x4*>(X + ii * G.ldx + (jt0 + j) * 16 + 4 * lg) =
+            (f16x4){(f16)x[i][j][0], (f16)x[i][j][1], (f16)x[i][j][2], (f16)x[i][j][3]};
+      }
+  };
+  if constexpr (!MOM) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[i][j][r] = ldexpf(x[i][j][r], inv_exp) * inv;
+      }
+  }
+  put_hi();
+
+  constexpr int NB2 = MT / 2, BLOCKS = NB2 * (NB2 + 1) / 2, S = MT == 2 ? 4 : MT == 4 ? 2 : 1;
+  constexpr int ROUNDS = (BLOCKS * S + SMALL_WAVES - 1) / SMALL_WAVES;
+  for (int step = 0; step < steps; ++step) {
+    __syncthreads();  // X written
+    f32x4 blk[ROUNDS][2][2];
+    // unit u = (block, slice of the contraction): rows 32 bi .., columns 32 bj .. of A, bj <= bi
+    auto unit = [&](int u, int& bi, int& bj, int& sl) {
+      const int k = u % BLOCKS;
+      sl = u / BLOCKS;
+      bi = k < 1 ? 0 : k < 3 ? 1 : k < 6 ? 2 : 3;
+      bj = k - bi * (bi + 1) / 2;
+    };
+    auto product = [&](const f16* src, int ld, int bi, int bj, int k0, int k1, f32x4 (&c)[2][2]) {
+      src += opaque0();
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) c[p][q] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      const f16 *rp = src + (bi * 32 + l15) * ld + 8 * lg, *rq = src + (bj * 32 + l15) * ld + 8 * lg;
+#pragma unroll 2
+      for (int k = k0; k < k1; k += 32) {
+        f16x8 vp[2], vq[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          vp[t] = *reinterpret_cast<const f16x8*>(rp + t * 16 * ld + k);
+          vq[t] = *reinterpret_cast<const f16x8*>(rq + t * 16 * ld + k);
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) c[p][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vp[p], vq[q], c[p][q], 0, 0, 0);
+      }
+    };
+#pragma unroll
+    for (int n = 0; n < ROUNDS; ++n) {
+      const int u = wave + n * SMALL_WAVES;
+      if (u >= BLOCKS * S) continue;
+      int bi, bj, sl;
+      unit(u, bi, bj, sl);
+      const int nk = np / 32;
+      product(X, G.ldx, bi, bj, nk * sl / S * 32, nk * (sl + 1) / S * 32, blk[n]);
+      if (S > 1 && sl > 0) {
+        float* to = scr + ((sl - 1) * BLOCKS + u % BLOCKS) * 1024 + lane * 4;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) *reinterpret_cast<f32x4*>(to + (p * 2 + q) * 256) = blk[n][p][q];
+      }
+    }
+    if (S > 1) __syncthreads();
+#pragma unroll
+    for (int n = 0; n < ROUNDS; ++n) {
+      const int u = wave + n * SMALL_WAVES;
+      if (u >= BLOCKS) continue;  // slice 0
+      int bi, bj, sl;
+      unit(u, bi, bj, sl);
+      const int oo = opaque0();
+      if (S > 1) {
+#pragma unroll
+        for (int k = 1; k < S; ++k)
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              blk[n][p][q] += *reinterpret_cast<const f32x4*>(scr + ((k - 1) * BLOCKS + u) * 1024 + lane * 4 + (p * 2 + q) * 256);
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int pp = oo + bi * 32 + p * 16 + 4 * lg, qq = bj * 32 + q * 16 + l15;
+          f16x4 h;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float v = blk[n][p][q][r];
+            h[r] = pp + r < m && qq < m && pp + r != qq ? (f16)(v * (SA / (SX * SX))) : (f16)0.f;
+            if (pp + r == qq) dA[qq] = qq < m ? v * (1.f / (SX * SX)) : 0.f;
+          }
+          *reinterpret_cast<f16x4*>(A + qq * G.lda + pp) = h;
+          if (bi != bj) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) A[(pp + r) * G.lda + qq] = h[r];
+          }
+        }
+    }
+    __syncthreads();  // A written
+#pragma unroll
+    for (int n = 0; n < ROUNDS; ++n) {
+      const int u = wave + n * SMALL_WAVES;
+      if (u >= BLOCKS) continue;
+      int bi, bj, sl;
+      unit(u, bi, bj, sl);
+      const int oo = opaque0();
+      product(A, G.lda, bi, bj, 0, mp, blk[n]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int pp = oo + bi * 32 + p * 16 + 4 * lg, qq = bj * 32 + q * 16 + l15;
+          const f16x4 o = *reinterpret_cast<const f16x4*>(A + qq * G.lda + pp);
+          const f32x4 dp = *reinterpret_cast<const f32x4*>(dA + pp);
+          const float dq = dA[qq];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float a = (float)o[r] * (1.f / SA), sq = blk[n][p][q][r] * (1.f / (SA * SA));
+            if (pp + r == qq) {
+              dB[qq] = QB * dq + QC * (sq + dq * dq);
+              blk[n][p][q][r] = 0.f;
+            } else {
+              blk[n][p][q][r] = (QB * a + QC * (sq + (dp[r] + dq) * a)) * SB;
+            }
+          }
+        }
+    }
+    __syncthreads();  // A read
+#pragma unroll
+    for (int n = 0; n < ROUNDS; ++n) {
+      const int u = wave + n * SMALL_WAVES;
+      if (u >= BLOCKS) continue;
+      int bi, bj, sl;
+      unit(u, bi, bj, sl);
+      const int oo = opaque0();
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int pp = oo + bi * 32 + p * 16 + 4 * lg, qq = bj * 32 + q * 16 + l15;
+          const f32x4 v = blk[n][p][q];
+          const f16x4 h = {(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+          *reinterpret_cast<f16x4*>(A + qq * G.lda + b_perm(pp)) = h;
+          if (bi != bj) {
+            const int qp = b_perm(qq);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) A[(pp + r) * G.lda + qp] = h[r];
+          }
+        }
+    }
+    __syncthreads();  // B written
+    const int o3 = opaque0();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      const float e = dB[i * 16 + l15 + o3];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[i][j][r] = (QA * x[i][j][r] + e * (float)(f16)x[i][j][r]) * SB;
+    }
+#pragma unroll
+    for (int k = 0; k < MT / 2; ++k) {
+      __builtin_amdgcn_sched_barrier(0);
+      f16x8 vb[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) vb[i] = *reinterpret_cast<const f16x8*>(A + (i * 16 + l15 + o3) * G.lda + k * 32 + 8 * lg);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        if (j >= njw || jt0 + j >= ntj) continue;
+        const f16* at = X + (k * 32 + 4 * lg + q4 + o3) * G.ldx + (jt0 + j) * 16 + 4 * p4;
+        const f16x4 x0 = read_tr(at), x1 = read_tr(at + 16 * G.ldx);
+        const f16x8 vx = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vx, vb[i], x[i][j], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) x[i][j] *= 1.f / SB;
+    if (step + 1 < steps) put_hi();
+  }
+
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      if (j >= njw || jt0 + j >= ntj) continue;
+      __builtin_amdgcn_sched_barrier(0);
+      const int ii = i * 16 + l15 + opaque0(), jj = (jt0 + j) * 16;
+      if constexpr (MOM) {
+        f16x4 h, l;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          h[r] = (f16)x[i][j][r];
+          l[r] = (f16)(x[i][j][r] - (float)h[r]);
+        }
+        *reinterpret_cast<f16x4*>(W.hi(0) + (size_t)ii * np + jj + 4 * lg) = h;
+        *reinterpret_cast<f16x4*>(W.lo + lo_tile(i * 16, jj, np) + lane * 8 + (jj >> 4 & 1) * 4) = l;
+      } else {
+        const f32x4 o = x[i][j] * (1.f / SX);
+        const uint2 u = otype == SWG_BF16 ? pack_bf16x4(o[0], o[1], o[2], o[3])
+                                          : __builtin_bit_cast(uint2, (f16x4){(f16)o[0], (f16)o[1], (f16)o[2], (f16)o[3]});
+        store4((uint16_t*)I.dst + (int64_t)b * I.bs_dst, I, I.ld_dst, tall, ii, jj + 4 * lg, __builtin_bit_cast(u16x4, u));
+      }
+    }
+}
+
+template <class T, bool MOM>
+__global__ __launch_bounds__(512, 1) void k_orth_small(const Item* __restrict__ items, const int32_t* __restrict__ ends,
+                                                       int count, int steps, double eps, int otype, char* __restrict__ ws) {
+  extern __shared__ __attribute__((aligned(1024))) char dyn[];
+  int first;
+  const int it = find_item(ends, count, blockIdx.x, first);
+  const Item& I = items[it];
+  const int b = blockIdx.x - first;
+  // by rows and by column tiles a wave holds: the fewer, the fewer registers
+  const int njw = (I.np / 16 + SMALL_WAVES - 1) / SMALL_WAVES;
+  switch (I.mp + (njw <= 2 ? 0 : njw <= 3 ? 1 : 2)) {
+    case 32: small_body<T, MOM, 2, 2>(I, b, steps, eps, otype, ws, dyn); break;
+    case 33: small_body<T, MOM, 2, 3>(I, b, steps, eps, otype, ws, dyn); break;
+    case 34: small_body<T, MOM, 2, 16>(I, b, steps, eps, otype, ws, dyn); break;
+    case 64: small_body<T, MOM, 4, 2>(I, b, steps, eps, otype, ws, dyn); break;
+    case 65: small_body<T, MOM, 4, 3>(I, b, steps, eps, otype, ws, dyn); break;
+    case 66: small_body<T, MOM, 4, 8>(I, b, steps, eps, otype, ws, dyn); break;
+    case 96: small_body<T, MOM, 6, 2>(I, b, steps, eps, otype, ws, dyn); break;
+    case 97: small_body<T, MOM, 6, 3>(I, b, steps, eps, otype, ws, dyn); break;
+    case 98: small_body<T, MOM, 6, 5>(I, b, steps, eps, otype, ws, dyn); break;
+    case 128: small_body<T, MOM, 8, 2>(I, b, steps, eps, otype, ws, dyn); break;
+    default: small_body<T, MOM, 8, 3>(I, b, steps, eps, otype, ws, dyn); break;
   }
 }
 
@@ -679,8 +1125,10 @@ constexpr int SQNORM_BLOCKS = 1024;
 // ---- host ----------------------------------------------------------------------------------------------------------
 // What a call over a list of shapes needs; the same arithmetic sizes the workspace, fills the table and sizes the grids
 struct Plan {
-  int count = 0, wt_sym = 2, wt_full = 2;  // tile sides / 32
-  int64_t grid[PREFIXES] = {0, 0, 0, 0, 0};
+  int count = 0, wt_full = 2;  // tile side of the X product / 32
+  int small_lds = 0;
+  bool all_small = true, use_small = true;
+  int64_t grid[PREFIXES] = {};
   int64_t parts = 0;
   size_t bytes = 0;                            // of X, A, B and the diagonals of all matrices
   double flops = 0;
@@ -688,8 +1136,9 @@ struct Plan {
 
 int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// tile side of each product: 128 where that gives at least 1.5 workgroups a CU, else 64
-bool plan_item(Plan& P, int32_t rows, int32_t cols, int32_t batch, Item* I) {
+// Small matrices take the one-workgroup form if the whole call does: beside larger ones the launches are there anyway, and
+// more workgroups share the work.  Tile side of each product: 128 where that gives at least 1.5 workgroups a CU, else 64
+bool plan_item(Plan& P, int32_t rows, int32_t cols, int32_t batch, bool mom, Item* I) {
   if (rows < 0 || cols < 0 || batch < 0 || rows > (1 << 20) || cols > (1 << 20)) return false;
   Item i = {};
   i.rows = rows; i.cols = cols; i.batch = batch;
@@ -704,41 +1153,53 @@ bool plan_item(Plan& P, int32_t rows, int32_t cols, int32_t batch, Item* I) {
   if (i.parts < 1) i.parts = 1;
   i.part_off = P.parts;
   i.off = (int64_t)P.bytes;
-  i.stride = (int64_t)align256((size_t)3 * i.mp * i.np * 2 + (size_t)2 * i.mp * i.mp * 2 + (size_t)2 * i.mp * 4);
-  P.parts += (int64_t)i.batch * i.parts;
+  if (i.batch && !is_small(i.m, i.mp, i.np)) P.all_small = false;
+  i.small = P.use_small && is_small(i.m, i.mp, i.np);
+  if (i.small) {
+    const int lds = small_geom(i.m, i.mp, i.np).bytes;
+    if (i.batch && lds > P.small_lds) P.small_lds = lds;
+  }
+  if (!i.small || mom) {
+    i.stride = (int64_t)align256((size_t)3 * i.mp * i.np * 2 + (size_t)2 * i.mp * i.mp * 2 + (size_t)2 * i.mp * 4);
+    P.parts += (int64_t)i.batch * i.parts;
+  }
   P.bytes += (size_t)i.batch * (size_t)i.stride;
   P.flops += (double)i.batch * (3.0 * i.m * i.m * (double)i.n + (double)i.m * i.m * (double)i.m);
   P.count += 1;
   if (I) *I = i;
   return true;
 }
-void plan_grids(const Item& i, int wt_sym, int wt_full, int64_t* g) {
-  const int64_t nt = cdiv64(i.mp, 32 * wt_sym), b = i.batch;
+void plan_grids(const Item& i, int wt_full, bool mom, int64_t* g) {
+  const int64_t nt = cdiv64(i.mp, SYM_TILE), b = i.batch, full = b * cdiv64(i.mp, 32 * wt_full) * cdiv64(i.np, 32 * wt_full);
+  if (i.small) g[P_SMALL] += b;
+  if (i.small && !mom) return;  // reads G and writes O by itself
   g[P_NORM] += b * i.parts;
   g[P_INIT] += b * cdiv64(i.mp, INIT_TILE) * cdiv64(i.np, INIT_TILE);
+  g[P_LAST] += full;
+  if (i.small) return;
   g[P_SYM] += b * (nt * (nt + 1) / 2);
-  g[P_FULL] += b * cdiv64(i.mp, 32 * wt_full) * cdiv64(i.np, 32 * wt_full);
+  g[P_FULL] += full;
 }
 
 // plan buffer (device): Item[count], int32 ends[PREFIXES][count], then the fp64 partial sums
 size_t table_bytes(int count) { return align256((size_t)count * sizeof(Item)) + align256((size_t)count * PREFIXES * 4); }
 
 template <class F>
-bool make_plan(int32_t count, F shape, Plan& P) {  // shape(i, rows, cols, batch)
+bool make_plan(int32_t count, bool mom, F shape, Plan& P) {  // shape(i, rows, cols, batch)
   if (count < 0) return false;
   for (int pass = 0; pass < 2; ++pass) {
-    P.parts = 0; P.bytes = 0; P.flops = 0; P.count = 0;
+    P.parts = 0; P.bytes = 0; P.flops = 0; P.count = 0; P.small_lds = 0;
     for (int k = 0; k < PREFIXES; ++k) P.grid[k] = 0;
     for (int32_t i = 0; i < count; ++i) {
       int32_t r, c, b;
       shape(i, r, c, b);
       Item it;
-      if (!plan_item(P, r, c, b, &it)) return false;
-      plan_grids(it, pass == 0 ? 4 : P.wt_sym, pass == 0 ? 4 : P.wt_full, P.grid);
+      if (!plan_item(P, r, c, b, mom, &it)) return false;
+      plan_grids(it, pass == 0 ? 4 : P.wt_full, mom, P.grid);
     }
     if (pass == 0) {
-      P.wt_sym = P.grid[P_SYM] >= 384 ? 4 : 2;
-      P.wt_full = P.grid[P_FULL] >= 384 ? 4 : 2;
+      P.use_small = P.all_small;
+      P.wt_full = P.grid[P_LAST] >= 384 ? 4 : 2;
     }
   }
   for (int k = 0; k < PREFIXES; ++k)
@@ -747,17 +1208,18 @@ bool make_plan(int32_t count, F shape, Plan& P) {  // shape(i, rows, cols, batch
 }
 
 template <class F>
-int write_table(int32_t count, const Plan& P, F fill, void* table, hipStream_t s) {  // fill(i, item): the caller's fields
+int write_table(int32_t count, const Plan& P, bool mom, F fill, void* table, hipStream_t s) {  // fill(i, item): the caller's fields
   Item* items = (Item*)table;
   int32_t* ends = (int32_t*)((char*)table + align256((size_t)count * sizeof(Item)));
   Plan run;
-  int64_t g[PREFIXES] = {0, 0, 0, 0, 0};
+  run.use_small = P.use_small;
+  int64_t g[PREFIXES] = {};
   for (int first = 0; first < count; first += TABLE_BATCH) {
     EntryBatch eb;
     const int n = count - first < TABLE_BATCH ? count - first : TABLE_BATCH;
     for (int k = 0; k < n; ++k) {
       fill(first + k, run, eb.e[k].item);
-      plan_grids(eb.e[k].item, P.wt_sym, P.wt_full, g);
+      plan_grids(eb.e[k].item, P.wt_full, mom, g);
       for (int q = 0; q < PREFIXES; ++q) eb.e[k].end[q] = (int32_t)g[q];
     }
     hipLaunchKernelGGL(k_orth_table, dim3(1), dim3(64), 0, s, eb, first, n, count, items, ends);
@@ -774,7 +1236,7 @@ struct Ptrs {
   int count;
   const int32_t* end(int k) const { return ends + (size_t)k * count; }
 };
-size_t ws_bytes_of(const Plan& P) { return align256((size_t)P.parts * 8) + P.bytes; }
+size_t ws_bytes_of(const Plan& P) { return align256((size_t)P.parts * 8) + P.bytes + 256; }
 Ptrs ptrs_of(int count, const Plan& P, const void* table, void* ws) {
   Ptrs r;
   r.items = (const Item*)table;
@@ -787,19 +1249,18 @@ Ptrs ptrs_of(int count, const Plan& P, const void* table, void* ws) {
 
 template <int MODE, int WT, int NB>
 void apply(const Plan& P, const Ptrs& p, int cur, int otype, const Momentum& mo, hipStream_t s) {
-  hipLaunchKernelGGL((k_orth_apply<MODE, WT, NB>), dim3((unsigned)P.grid[P_FULL]), dim3(256), 0, s, p.items, p.end(P_FULL),
-                     p.count, cur, otype, p.ws, mo);
+  constexpr int G = MODE == MID ? P_FULL : P_LAST;
+  hipLaunchKernelGGL((k_orth_apply<MODE, WT, NB>), dim3((unsigned)P.grid[G]), dim3(256), 0, s, p.items, p.end(G), p.count, cur,
+                     otype, p.ws, mo);
 }
 template <int MODE>
 int run_steps(const Plan& P, const Ptrs& p, int steps, int otype, const Momentum& mo, hipStream_t s) {
   const dim3 gs((unsigned)P.grid[P_SYM]);
-  for (int k = 0, cur = 0; k < steps; ++k, cur ^= 1) {
-    if (P.wt_sym == 4) {
-      hipLaunchKernelGGL((k_orth_sym<true, 4, 2>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
-      hipLaunchKernelGGL((k_orth_sym<false, 4, 2>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
-    } else {
-      hipLaunchKernelGGL((k_orth_sym<true, 2, 3>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
-      hipLaunchKernelGGL((k_orth_sym<false, 2, 3>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
+  const bool only_last = P.grid[P_FULL] == 0;  // small matrices alone: their steps are made
+  for (int k = only_last ? steps - 1 : 0, cur = 0; k < steps; ++k, cur ^= 1) {
+    if (!only_last) {
+      hipLaunchKernelGGL((k_orth_sym<true, 2, 2>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
+      hipLaunchKernelGGL((k_orth_sym<false, 2, 2>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
     }
     if (k + 1 < steps) {
       if (P.wt_full == 4) apply<MID, 4, 2>(P, p, cur, otype, mo, s);
@@ -814,14 +1275,22 @@ int run_steps(const Plan& P, const Ptrs& p, int steps, int otype, const Momentum
 }
 
 template <class T, bool MOM>
-int run_init(const Plan& P, const Ptrs& p, float eps, const Momentum& mo, hipStream_t s) {
-  hipLaunchKernelGGL((k_orth_norm<T, MOM>), dim3((unsigned)P.grid[P_NORM]), dim3(256), 0, s, p.items, p.end(P_NORM), p.count,
-                     p.part, mo);
-  SWG_LAUNCH_CHECK();
-  hipLaunchKernelGGL((k_orth_init<T, MOM>), dim3((unsigned)P.grid[P_INIT]), dim3(256), 0, s, p.items, p.end(P_INIT), p.count,
-                     p.part, (double)eps, p.ws, mo);
-  SWG_LAUNCH_CHECK();
-  return 0;
+int run_all(const Plan& P, const Ptrs& p, int steps, int otype, float eps, const Momentum& mo, hipStream_t s) {
+  if (P.grid[P_NORM]) {
+    hipLaunchKernelGGL((k_orth_norm<T, MOM>), dim3((unsigned)P.grid[P_NORM]), dim3(256), 0, s, p.items, p.end(P_NORM), p.count,
+                       p.part, mo);
+    hipLaunchKernelGGL((k_orth_init<T, MOM>), dim3((unsigned)P.grid[P_INIT]), dim3(256), 0, s, p.items, p.end(P_INIT), p.count,
+                       p.part, (double)eps, p.ws, mo);
+    SWG_LAUNCH_CHECK();
+  }
+  if (P.grid[P_SMALL]) {
+    static std::atomic<uint64_t> ready{0};
+    if (int e = ensure_dyn_lds(ready, (const void*)k_orth_small<T, MOM>, SMALL_LDS)) return e;
+    hipLaunchKernelGGL((k_orth_small<T, MOM>), dim3((unsigned)P.grid[P_SMALL]), dim3(512), P.small_lds, s, p.items,
+                       p.end(P_SMALL), p.count, steps, (double)eps, otype, p.ws);
+    SWG_LAUNCH_CHECK();
+  }
+  return P.grid[P_LAST] ? run_steps<MOM ? STEP : OUT>(P, p, steps, otype, mo, s) : 0;
 }
 
 }  // namespace
@@ -831,7 +1300,7 @@ extern "C" {
 size_t swg_orthogonalise_workspace_bytes(int32_t count, const swg_orth_item* items) {
   if (count <= 0 || !items) return 0;
   Plan P;
-  if (!make_plan(count, [&](int i, int32_t& r, int32_t& c, int32_t& b) { r = items[i].rows; c = items[i].cols; b = items[i].batch; }, P))
+  if (!make_plan(count, false, [&](int i, int32_t& r, int32_t& c, int32_t& b) { r = items[i].rows; c = items[i].cols; b = items[i].batch; }, P))
     return 0;
   return table_bytes(count) + ws_bytes_of(P) + 256;
 }
@@ -843,7 +1312,7 @@ int swg_orthogonalise(int32_t count, const swg_orth_item* items, int32_t itype, 
   if (!items) return SWG_E_NULL;
   if (itype < SWG_F32 || itype > SWG_F16 || (otype != SWG_BF16 && otype != SWG_F16)) return SWG_E_UNSUPPORTED;
   Plan P;
-  if (!make_plan(count, [&](int i, int32_t& r, int32_t& c, int32_t& b) { r = items[i].rows; c = items[i].cols; b = items[i].batch; }, P))
+  if (!make_plan(count, false, [&](int i, int32_t& r, int32_t& c, int32_t& b) { r = items[i].rows; c = items[i].cols; b = items[i].batch; }, P))
     return SWG_E_SHAPE;
   for (int i = 0; i < count; ++i) {
     const swg_orth_item& e = items[i];
@@ -851,29 +1320,27 @@ int swg_orthogonalise(int32_t count, const swg_orth_item* items, int32_t itype, 
     if (!e.g || !e.out) return SWG_E_NULL;
     if (e.ld_g < e.cols || e.ld_out < e.cols) return SWG_E_SHAPE;
   }
-  if (P.grid[P_FULL] == 0) return 0;
+  if (P.grid[P_LAST] + P.grid[P_SMALL] == 0) return 0;
   if (!ws) return SWG_E_NULL;
   if (ws_bytes < table_bytes(count) + ws_bytes_of(P) + 256) return SWG_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   void* table = (void*)(((size_t)ws + 255) & ~(size_t)255);
   SwgProfScope ps(KID_ORTH, P.flops * steps, 0.0, s);
-  int r = write_table(count, P, [&](int i, Plan& run, Item& I) {
+  int r = write_table(count, P, false, [&](int i, Plan& run, Item& I) {
     const swg_orth_item& e = items[i];
-    plan_item(run, e.rows, e.cols, e.batch, &I);
+    plan_item(run, e.rows, e.cols, e.batch, false, &I);
     I.src = e.g; I.dst = e.out; I.ld_src = e.ld_g; I.bs_src = e.bs_g; I.ld_dst = e.ld_out; I.bs_dst = e.bs_out;
   }, table, s);
   if (r) return r;
   const Ptrs p = ptrs_of(count, P, table, (char*)table + table_bytes(count));
   const Momentum none = {};
-  if (itype == SWG_F32) r = run_init<float, false>(P, p, eps, none, s);
-  else if (itype == SWG_BF16) r = run_init<bf16, false>(P, p, eps, none, s);
-  else r = run_init<f16, false>(P, p, eps, none, s);
-  if (r) return r;
-  return run_steps<OUT>(P, p, steps, otype, none, s);
+  if (itype == SWG_F32) return run_all<float, false>(P, p, steps, otype, eps, none, s);
+  if (itype == SWG_BF16) return run_all<bf16, false>(P, p, steps, otype, eps, none, s);
+  return run_all<f16, false>(P, p, steps, otype, eps, none, s);
 }
 
 static bool muon_plan(int32_t count, const swg_muon_item* items, Plan& P) {
-  return make_plan(count, [&](int i, int32_t& r, int32_t& c, int32_t& b) { r = items[i].rows; c = items[i].cols; b = 1; }, P);
+  return make_plan(count, true, [&](int i, int32_t& r, int32_t& c, int32_t& b) { r = items[i].rows; c = items[i].cols; b = 1; }, P);
 }
 
 size_t swg_muon_table_bytes(int32_t count) { return count <= 0 ? 0 : table_bytes(count); }
@@ -892,8 +1359,8 @@ int swg_muon_table(int32_t count, const swg_muon_item* items, void* table, size_
   for (int i = 0; i < count; ++i)
     if (items[i].rows < 1 || items[i].cols < 1 || items[i].flat_off < 0 || items[i].index < 0) return SWG_E_SHAPE;
   if (table_size < table_bytes(count)) return SWG_E_WORKSPACE;
-  return write_table(count, P, [&](int i, Plan& run, Item& I) {
-    plan_item(run, items[i].rows, items[i].cols, 1, &I);
+  return write_table(count, P, true, [&](int i, Plan& run, Item& I) {
+    plan_item(run, items[i].rows, items[i].cols, 1, true, &I);
     I.flat_off = items[i].flat_off; I.index = items[i].index; I.scale = items[i].scale;
   }, table, (hipStream_t)stream);
 }
@@ -915,8 +1382,7 @@ int swg_muon_ema_step(int32_t count, const swg_muon_item* items, const void* tab
   for (int k = 0; k < n_ema; ++k) mo.ema_w[k] = 1.0f - ema_decay[k];
   SwgProfScope ps(KID_ORTH, P.flops * steps, 0.0, s);
   const Ptrs p = ptrs_of(count, P, table, ws);
-  if (int r = run_init<float, true>(P, p, eps, mo, s)) return r;
-  return run_steps<STEP>(P, p, steps, 0, mo, s);
+  return run_all<float, true>(P, p, steps, 0, eps, mo, s);
 }
 
 size_t swg_grad_sqnorm_ordered_workspace_bytes(void) { return SQNORM_BLOCKS * sizeof(double); }

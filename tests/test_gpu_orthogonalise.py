@@ -37,7 +37,10 @@ def _check(g, out, steps=5, eps=1e-7):
 # below, at and beyond the 32-wide padding, the 64- and 128-wide tiles, the transposed orientation of each
 SHAPES = [(1, 1), (1, 7), (7, 1), (2, 3), (1, 1000), (1000, 1), (31, 33), (32, 32), (33, 31), (33, 65), (60, 60), (60, 240), (64, 64),
           (65, 64), (96, 96), (96, 384), (384, 96), (120, 120), (129, 127), (127, 300), (192, 512), (251, 1003), (1003, 251),
-          (257, 257), (40, 4099), (768, 512)]
+          (257, 257), (40, 4099), (768, 512),
+          # the one-workgroup form: each row class, its column classes and their ends, and just beyond them
+          (20, 2048), (20, 2049), (32, 256), (300, 30), (32, 385), (64, 256), (64, 384), (64, 960), (1000, 60), (90, 600), (96, 640),
+          (641, 96), (70, 386), (128, 256), (100, 257), (128, 384), (120, 360), (384, 121), (128, 385)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -186,10 +189,13 @@ def test_streams_and_captured_graphs():
 
 
 # ---- FusedMuonEMA ------------------------------------------------------------------------------------------------------
-def _network(seed):
+def _network(seed, big=False):
+    """Parameters and how many of them are matrices; `big`: with matrices that only the many-launch form takes."""
     g = torch.Generator(device=DEV).manual_seed(seed)
-    shapes = [(96, 96), (288, 96), (96, 384), (17, 5), (1, 30), (61, 250), (250, 61), (95,), (96,), (3, 4, 5), (1,), (2100,)]
-    return [torch.nn.Parameter(0.05 * torch.randn(*s, device=DEV, generator=g)) for s in shapes], 7
+    shapes = [(96, 96), (288, 96), (96, 384), (17, 5), (1, 30), (61, 250), (250, 61)] + ([(200, 301), (513, 140)] if big else [])
+    k = len(shapes)
+    shapes += [(95,), (96,), (3, 4, 5), (1,), (2100,)]
+    return [torch.nn.Parameter(0.05 * torch.randn(*s, device=DEV, generator=g)) for s in shapes], k
 
 
 def _grads(params, seed, f=1e-2):
@@ -229,11 +235,12 @@ def _reference_step(st, k, grads, lr, mu, nesterov, wd, steps, max_norm, betas, 
 
 @pytest.mark.parametrize("kw", [dict(), dict(nesterov=False, weight_decay=0.1), dict(max_norm=0.5, ema_betas=(0.9, 0.99)),
                                 dict(ns_steps=3, momentum=0.0, ema_betas=(0.5,) * 8, weight_decay=0.01), dict(max_norm=1e9)])
-def test_optimizer_steps(kw):
+@pytest.mark.parametrize("big", [False, True])
+def test_optimizer_steps(kw, big):
     """Four steps against float64.  m, v: 4 roundings a step, 16 u in all of values that only grow; p: those of the update
     (the emulation's bound, added up over the steps) and 4 u |p| a step; Adam's quotient 16 u of its size lr / (1 - b1)."""
     import swingnn_amd as S
-    params, k = _network(1)
+    params, k = _network(1, big)
     lr = 2e-3
     opt = S.FusedMuonEMA(params[:k], params[k:], lr=lr, **kw)
     st = {"t": 0, "p": [p.detach().double().clone() for p in params], "m": [torch.zeros_like(p, dtype=torch.float64) for p in params],
@@ -270,12 +277,13 @@ def test_optimizer_steps(kw):
             assert float((e - st["ema"][j][i]).abs().max()) <= bound + 16 * u, (i, j)
 
 
-def test_optimizer_repeats_itself_and_resumes():
+@pytest.mark.parametrize("big", [False, True])
+def test_optimizer_repeats_itself_and_resumes(big):
     """Equal runs give equal bits; a run resumed from its checkpoint goes on as the uninterrupted one."""
     import swingnn_amd as S
     runs = []
     for resume in (False, False, True):
-        params, k = _network(3)
+        params, k = _network(3, big)
         opt = S.FusedMuonEMA(params[:k], params[k:], lr=1e-3, max_norm=1.0, ema_betas=(0.9, 0.99))
         for step in range(5):
             if resume and step == 3:
