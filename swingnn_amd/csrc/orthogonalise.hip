@@ -705,30 +705,26 @@ __global__ __launch_bounds__(256, 2) void k_orth_apply(const Item* __restrict__ 
 // steps, this form / the launches: 32 x 32 21 / 49 us, 96 x 96 32 / 65, 60 x 240 30 / 66, 96 x 384 47 / 77, 128 x 384 77 / 80,
 // 32 x 2048 79 / 122, 512 of 96 x 96 66 / 180; a fourth column tile a wave at 128 rows spills (120 x 512: 112 / 86).
 struct SmallGeom {
-  int mr, ldx, lda;       // rows of X kept in LDS, row strides (elements) of X and A
+  int ldx, lda;  // row strides (elements) of X and A
   int off_a, off_d, off_red, bytes;
 };
 constexpr int SMALL_LDS = 163840, SMALL_WAVES = 8;
 // number of waves that share the contraction of a 32 x 32 block of A
 __host__ __device__ inline int small_split(int mp) { return mp == 32 ? 4 : mp == 64 ? 2 : 1; }
-__host__ __device__ inline SmallGeom small_geom(int m, int mp, int np) {
+__host__ __device__ inline SmallGeom small_geom(int mp, int np) {
   SmallGeom g;
   g.ldx = np + 8;  // 16 bytes more than a multiple of the banks: the 16 rows of a fragment read spread over them
   g.lda = mp + 8;
   const int a = mp * g.lda * 2, nb = mp / 32, blocks = nb * (nb + 1) / 2;
-  const int rest = a + 2 * mp * 4 + blocks * (small_split(mp) - 1) * 4096 + 64;
-  g.mr = mp;
-  // X's rows behind m are only ever multiplied by zeros of B or left out: they may lie in A's place, which is finite
-  if (mp * g.ldx * 2 + rest > SMALL_LDS && (mp - ((m + 7) & ~7)) * g.ldx * 2 <= a) g.mr = (m + 7) & ~7;
-  g.off_a = g.mr * g.ldx * 2;
+  g.off_a = mp * g.ldx * 2;
   g.off_d = g.off_a + a;
   g.off_red = g.off_d + 2 * mp * 4;
-  g.bytes = g.off_a + rest;
+  g.bytes = g.off_red + blocks * (small_split(mp) - 1) * 4096 + SMALL_WAVES * 8;
   return g;
 }
 __host__ __device__ inline int small_nj(int mt) { return mt == 2 ? 16 : mt == 4 ? 8 : mt == 6 ? 5 : 3; }  // column tiles a wave holds
-inline bool is_small(int m, int mp, int np) {
-  return mp <= 128 && (np / 16 + SMALL_WAVES - 1) / SMALL_WAVES <= small_nj(mp / 16) && small_geom(m, mp, np).bytes <= SMALL_LDS;
+inline bool is_small(int mp, int np) {
+  return mp <= 128 && (np / 16 + SMALL_WAVES - 1) / SMALL_WAVES <= small_nj(mp / 16) && small_geom(mp, np).bytes <= SMALL_LDS;
 }
 
 // 0 that the compiler cannot see through: addresses formed with it are not kept in registers over the steps, where the
@@ -778,7 +774,7 @@ __device__ __forceinline__ void small_body(const Item& I, int b, int steps, doub
                                            char* lds) {
   const int m = I.m, mp = I.mp, np = I.np, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int l15 = lane & 15, lg = lane >> 4, q4 = l15 >> 2, p4 = l15 & 3;
-  const SmallGeom G = small_geom(m, mp, np);
+  const SmallGeom G = small_geom(mp, np);
   f16* X = (f16*)lds;
   f16* A = (f16*)(lds + G.off_a);
   float *dA = (float*)(lds + G.off_d), *dB = dA + mp;
@@ -846,7 +842,7 @@ __device__ __forceinline__ void small_body(const Item& I, int b, int steps, doub
       for (int j = 0; j < NJ; ++j) {
         const int ii = i * 16 + l15 + o;
         __builtin_amdgcn_sched_barrier(0);
-        if (j >= njw || jt0 + j >= ntj || ii >= G.mr) continue;
+        if (j >= njw || jt0 + j >= ntj) continue;
         *reinterpret_cast<f16x4*>(X + ii * G.ldx + (jt0 + j) * 16 + 4 * lg) =
             (f16x4){(f16)x[i][j][0], (f16)x[i][j][1], (f16)x[i][j][2], (f16)x[i][j][3]};
       }
@@ -1153,10 +1149,10 @@ bool plan_item(Plan& P, int32_t rows, int32_t cols, int32_t batch, bool mom, Ite
   if (i.parts < 1) i.parts = 1;
   i.part_off = P.parts;
   i.off = (int64_t)P.bytes;
-  if (i.batch && !is_small(i.m, i.mp, i.np)) P.all_small = false;
-  i.small = P.use_small && is_small(i.m, i.mp, i.np);
+  if (i.batch && !is_small(i.mp, i.np)) P.all_small = false;
+  i.small = P.use_small && is_small(i.mp, i.np);
   if (i.small) {
-    const int lds = small_geom(i.m, i.mp, i.np).bytes;
+    const int lds = small_geom(i.mp, i.np).bytes;
     if (i.batch && lds > P.small_lds) P.small_lds = lds;
   }
   if (!i.small || mom) {

@@ -21,11 +21,17 @@ _TYPE = {torch.float32: L.SWG_F32, torch.bfloat16: L.SWG_BF16, torch.float16: L.
 
 def _rows(t, D):
     """t as [rows, D] with unit stride along D, without a copy where its strides allow it."""
-    try:
-        t = t.view(-1, D)
-    except RuntimeError:
-        t = t.reshape(-1, D)
+    if t.dim() != 2:
+        try:
+            t = t.view(-1, D)
+        except RuntimeError:
+            t = t.reshape(-1, D)
     return t if D == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _like(t):
+    """An uninitialised contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _ptr(t):
@@ -36,45 +42,58 @@ def _forward(x, weight, bias, eps, keep):
     D = x.shape[-1]
     x2 = _rows(x, D)
     rows = x2.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
+    y = _like(x)
+    stat = mean = rstd = None
     if keep:
-        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        stat = x2.new_empty((2, rows), dtype=torch.float32)  # mean, then 1 / sqrt(var + eps)
+        mean = stat.data_ptr()
+        rstd = mean + 4 * rows
     wt = weight if weight is not None else bias
+    wtype = _TYPE[x.dtype if wt is None else wt.dtype]
     call_on(x.device, L.lib.swg_layer_norm_fwd, "swg_layer_norm_fwd", rows, D, x2.data_ptr(), x2.stride(0), _TYPE[x.dtype],
-            _ptr(weight), _ptr(bias), _TYPE[x.dtype if wt is None else wt.dtype], eps, y.data_ptr(), D, _ptr(mean),
-            _ptr(rstd))
-    return y, x2, mean, rstd
+            _ptr(weight), _ptr(bias), wtype, eps, y.data_ptr(), D, mean, rstd)
+    return y, x2, stat, wtype
+
+
+_WS_FLOATS = {}  # (rows, D, type) -> size: plain numbers, asked for once
+
+
+def _ws_floats(rows, D, xt):
+    n = _WS_FLOATS.get((rows, D, xt))
+    if n is None:
+        if len(_WS_FLOATS) > 4096:
+            _WS_FLOATS.clear()
+        n = _WS_FLOATS[(rows, D, xt)] = L.lib.swg_layer_norm_bwd_workspace_bytes(rows, D, xt) // 4
+    return n
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, x2, mean, rstd = _forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x2, weight, bias, mean, rstd)
+        y, x2, stat, ctx.wtype = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x2, weight, bias, stat)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x2, weight, bias, mean, rstd = ctx.saved_tensors
+        x2, weight, bias, stat = ctx.saved_tensors
         rows, D = x2.shape
-        shape, dev = dy.shape, x2.device
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        dx = _like(dy) if need_x else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty_like(bias) if need_b else None
         dy = _rows(dy, D)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty((rows, D), dtype=x2.dtype, device=dev) if need_x else None
-        dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w else None
-        db = torch.empty_like(bias, memory_format=torch.contiguous_format) if need_b else None
-        wt = weight if weight is not None else bias
         xt = _TYPE[x2.dtype]
         nbytes, ws = 0, None
         if need_w or need_b:
-            nbytes = L.lib.swg_layer_norm_bwd_workspace_bytes(rows, D, xt)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        call_on(dev, L.lib.swg_layer_norm_bwd, "swg_layer_norm_bwd", rows, D, x2.data_ptr(), x2.stride(0), dy.data_ptr(),
-                dy.stride(0), xt, _ptr(weight), xt if wt is None else _TYPE[wt.dtype], mean.data_ptr(), rstd.data_ptr(),
-                _ptr(dx), D, _ptr(dw), _ptr(db), _ptr(ws), nbytes)
-        return (None if dx is None else dx.view(shape)), dw, db, None
+            n = _ws_floats(rows, D, xt)
+            nbytes, ws = 4 * n, stat.new_empty(n)
+        mean = stat.data_ptr()
+        call_on(x2.device, L.lib.swg_layer_norm_bwd, "swg_layer_norm_bwd", rows, D, x2.data_ptr(), x2.stride(0), dy.data_ptr(),
+                dy.stride(0), xt, _ptr(weight), ctx.wtype, mean, mean + 4 * rows, _ptr(dx), D, _ptr(dw), _ptr(db), _ptr(ws),
+                nbytes)
+        return dx, dw, db, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):

@@ -73,6 +73,7 @@ class FusedAdamEMA(torch.optim.Optimizer):
         self._p_ptrs = torch.tensor(self._p_key, dtype=torch.int64, device=dev)
         self._g_ptrs = torch.zeros(len(self.params), dtype=torch.int64, device=dev)
         self._g_key = None
+        self._views = None
         self._sqnorm = torch.zeros(1, dtype=torch.float32, device=dev)
         self.step_count = 0
         self.ema_updates = 0
@@ -160,6 +161,7 @@ class FusedAdamEMA(torch.optim.Optimizer):
         if pkey != self._p_key:  # parameter storage moved (model.to(), p.data = ..., load_state_dict(assign=True))
             self._p_ptrs.copy_(torch.tensor(pkey, dtype=torch.int64), non_blocking=False)
             self._p_key = pkey
+            self._views = None
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -192,8 +194,11 @@ class FusedAdamEMA(torch.optim.Optimizer):
 
     def _bump_versions(self):
         """Parameters were updated through raw pointers; bump their version counters so derived weight caches
-        (engine.NetCache) rebuild: one foreach call on zero-size views (no element is touched, the counters move)."""
-        torch._foreach_add_([p.view(-1)[:0] for p in self.params], 0.0)
+        (engine.NetCache) rebuild: one foreach call on zero-size views (no element is touched, the counters move).  The
+        views are kept until a parameter's storage moves: making 392 of them took 560 us of a step, using them 37 us."""
+        if self._views is None:
+            self._views = [p.view(-1)[:0] for p in self.params]
+        torch._foreach_add_(self._views, 0.0)
 
 
 class FusedMuonEMA(FusedAdamEMA):
