@@ -487,8 +487,9 @@ int swg_layer_norm_bwd(int64_t rows, int32_t D, const void* x, int64_t ldx, cons
  *   u = nesterov ? momentum m + (1 - momentum) g : m;  p <- p (1 - lr weight_decay) - lr scale orthogonalise(u);
  *   ema_k <- lerp(ema_k, p, 1 - ema_decay[k]) (ema_decay: HOST array).  p, g: DEVICE pointer tables, contiguous fp32;
  *   m [total], ema [n_ema, total] at flat_off.  The matrix must not appear twice.
- * swg_grad_sqnorm_ordered: swg_grad_sqnorm with fp64 partial sums joined in a fixed order (equal inputs, equal bits) and
- *   without a memory clear, so it may be recorded into a graph. */
+ *   sqnorm (or NULL: no clip) is written first: the sum of squares of every gradient of the entries and of the other
+ *   parameters, whose chunks numel / chunk_tensor / chunk_off (n_chunks, may be 0) name as for swg_grad_sqnorm; fp64
+ *   partial sums joined in a fixed order (equal inputs, equal bits).  ws: 256-byte aligned. */
 typedef struct swg_orth_item {
   const void* g;
   void* out;
@@ -507,12 +508,10 @@ size_t swg_muon_table_bytes(int32_t count);
 int swg_muon_table(int32_t count, const swg_muon_item* items, void* table, size_t table_size, void* stream);
 size_t swg_muon_workspace_bytes(int32_t count, const swg_muon_item* items);
 int swg_muon_ema_step(int32_t count, const swg_muon_item* items, const void* table, const void* p_ptrs, const void* g_ptrs,
-                      float* m, float* ema, int64_t total, int32_t n_ema, const float* ema_decay, const float* sqnorm,
-                      float max_norm, float lr, float momentum, int32_t nesterov, float weight_decay, int32_t steps,
-                      float eps, void* ws, size_t ws_bytes, void* stream);
-size_t swg_grad_sqnorm_ordered_workspace_bytes(void);
-int swg_grad_sqnorm_ordered(const void* g_ptrs, const int32_t* numel, const int32_t* chunk_tensor, const int32_t* chunk_off,
-                            int32_t n_chunks, float* sqnorm, void* ws, size_t ws_bytes, void* stream);
+                      float* m, float* ema, int64_t total, int32_t n_ema, const float* ema_decay, const int32_t* numel,
+                      const int32_t* chunk_tensor, const int32_t* chunk_off, int32_t n_chunks, float* sqnorm, float max_norm,
+                      float lr, float momentum, int32_t nesterov, float weight_decay, int32_t steps, float eps, void* ws,
+                      size_t ws_bytes, void* stream);
 
 /* ---- post-sampling: attribute codecs of the molecule path -------------------------------- *
  * utils/attribute_code.py:14-329.  Node attributes [B,N] (int / ddpm) or [B,N,C] (one-hot / bits); adjacency

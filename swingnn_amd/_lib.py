@@ -185,9 +185,7 @@ SYMBOLS = {
     "swg_muon_table": (C.c_int, [_i32, C.POINTER(SwgMuonItem), _fp, _sz, _fp]),
     "swg_muon_workspace_bytes": (_sz, [_i32, C.POINTER(SwgMuonItem)]),
     "swg_muon_ema_step": (C.c_int, [_i32, C.POINTER(SwgMuonItem), _fp, _fp, _fp, _fp, _fp, _i64, _i32, C.POINTER(C.c_float),
-                                    _fp, _f, _f, _f, _i32, _f, _i32, _f, _fp, _sz, _fp]),
-    "swg_grad_sqnorm_ordered_workspace_bytes": (_sz, []),
-    "swg_grad_sqnorm_ordered": (C.c_int, [_fp, _fp, _fp, _fp, _i32, _fp, _fp, _sz, _fp]),
+                                    _fp, _fp, _fp, _i32, _fp, _f, _f, _f, _i32, _f, _i32, _f, _fp, _sz, _fp]),
     "swg_attr_decode": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _fp, _fp, _fp, _fp, _fp, _fp]),
     "swg_attr_encode": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _fp, _fp, _fp, _fp]),
     "swg_graph_stats_workspace_bytes": (_sz, [_i32, _i32]),

@@ -18,6 +18,7 @@
 // step (A, B, X).  A workgroup finds its matrix in a table of running tile counts (one load per lane and a ballot).
 // A and B are symmetric: the tiles on and below the diagonal are computed and written twice.
 #include "common.h"
+#include <type_traits>
 
 namespace {
 
@@ -54,9 +55,9 @@ struct Item {
   float scale;       // momentum form: update = lr scale O
   int32_t small;     // all steps in one workgroup
 };
-// running workgroup counts: norm, init, symmetric products, X product, whole small matrices, last X product
-constexpr int PREFIXES = 6;
-enum { P_NORM = 0, P_INIT, P_SYM, P_FULL, P_SMALL, P_LAST };
+// running workgroup counts: norm, init, tiles of A, tiles of B, X product, whole small matrices, last X product
+constexpr int PREFIXES = 7;
+enum { P_NORM = 0, P_INIT, P_GRAM, P_POLY, P_FULL, P_SMALL, P_LAST };
 struct Entry {
   Item item;
   int32_t end[PREFIXES];  // running totals including this item
@@ -127,6 +128,10 @@ struct Momentum {
   float max_norm, mu, lr, keep;  // keep = 1 - lr * weight_decay
   int32_t nesterov, n_ema;
   float ema_w[8];
+  // the other parameters' chunks (for the clip's norm) and their partial sums
+  const int32_t *numel, *chunk_tensor, *chunk_off;
+  double* others;
+  int32_t n_chunks, chunk;
 };
 
 __device__ __forceinline__ float clip_of(const Momentum& mo) {
@@ -154,44 +159,75 @@ __device__ __forceinline__ void swap_rows(f16x4& a, f16x4& b) {
 }
 __device__ __forceinline__ int swapped_col(int lg) { return 8 * (lg >> 1) + 16 * (lg & 1); }
 
-// sum of squares of a slice of a matrix into part[] (fp64: neither 1e-30 nor 1e30 leaves its range).  Momentum form: also
-// m <- mu m + (1 - mu) g, and the squares are the update's.
+__device__ __forceinline__ double block_sum(double s, double* red) {  // 256 threads; all get the sum
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = (red[0] + red[1]) + (red[2] + red[3]);
+  __syncthreads();
+  return s;
+}
+
+// Sums over a slice of a matrix into part[] (fp64: neither 1e-30 nor 1e30 leaves its range): |G|^2, or in the momentum form
+// |g|^2, <g, m> and |m|^2.  The update u = a m + b c g is linear in the old m and in g, so these three give |u| for any clip
+// factor c: the clip's norm and the updates' norms take one pass over g and m.  Workgroups behind the matrices' (momentum
+// form) sum |g|^2 of the other parameters.
 template <class T, bool MOM>
 __global__ __launch_bounds__(256) void k_orth_norm(const Item* __restrict__ items, const int32_t* __restrict__ ends,
-                                                   int count, double* __restrict__ part, Momentum mo) {
+                                                   int count, int blocks, double* __restrict__ part, Momentum mo) {
   __shared__ double red[4];
+  constexpr int N = 16 / (int)sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+  double s = 0.0, gm = 0.0, mm = 0.0;
+  if (MOM && (int)blockIdx.x >= blocks) {
+    const int wg = blockIdx.x - blocks, n_wg = gridDim.x - blocks;
+    for (int c = wg; c < mo.n_chunks; c += n_wg) {
+      const int t = mo.chunk_tensor[c], off = mo.chunk_off[c], n = min(mo.chunk, mo.numel[t] - off);
+      const float* g = mo.g_ptrs[t] + off;
+      for (int i = threadIdx.x; i < n; i += 256) s += (double)g[i] * (double)g[i];
+    }
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) mo.others[wg] = s;
+    return;
+  }
   int first;
   const int it = find_item(ends, count, blockIdx.x, first);
   const Item& I = items[it];
   const int w = blockIdx.x - first, b = w / I.parts, k = w - b * I.parts;
   const int64_t numel = (int64_t)I.rows * I.cols;
-  constexpr int N = 16 / (int)sizeof(T);
-  typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
   const int64_t per = ((numel + I.parts - 1) / I.parts + N - 1) / N * N;
   const int64_t lo = k * per, hi = lo + per < numel ? lo + per : numel;
-  double s = 0.0;
   if constexpr (MOM) {
     const float* g = mo.g_ptrs[I.index];
-    float* m = mo.m + I.flat_off;
-    const float clip = clip_of(mo);
+    const float* m = mo.m + I.flat_off;
     int64_t i = lo + threadIdx.x * N;
-    for (; i + N <= hi; i += 256 * N) {
-      const vec gv = *reinterpret_cast<const vec*>(g + i);
-      vec mv = *reinterpret_cast<const vec*>(m + i);
+    auto add = [&](const vec& gv, const vec& mv) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float c = gv[e] * clip;
-        mv[e] = new_m(mo, mv[e], c);
-        const double u = update_of(mo, mv[e], c);
-        s += u * u;
+        const double a = gv[e], c = mv[e];
+        s += a * a;
+        gm += a * c;
+        mm += c * c;
       }
-      *reinterpret_cast<vec*>(m + i) = mv;
+    };
+    constexpr int U = 4, W = 256 * N;  // U vectors of each in flight
+    for (; i + (U - 1) * W + N <= hi; i += U * W) {
+      vec gv[U], mv[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        gv[u] = *reinterpret_cast<const vec*>(g + i + u * W);
+        mv[u] = *reinterpret_cast<const vec*>(m + i + u * W);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) add(gv[u], mv[u]);
     }
+    for (; i + N <= hi; i += W) add(*reinterpret_cast<const vec*>(g + i), *reinterpret_cast<const vec*>(m + i));
     for (; i < hi; ++i) {  // fewer than N left: one lane's
-      const float c = g[i] * clip, mv = new_m(mo, m[i], c);
-      m[i] = mv;
-      const double u = update_of(mo, mv, c);
-      s += u * u;
+      const double a = g[i], c = m[i];
+      s += a * a;
+      gm += a * c;
+      mm += c * c;
     }
   } else {
     const T* g = (const T*)I.src + (int64_t)b * I.bs_src;
@@ -210,11 +246,28 @@ __global__ __launch_bounds__(256) void k_orth_norm(const Item* __restrict__ item
       for (; i < z; ++i) s += (double)(float)row[i] * (double)(float)row[i];
     }
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) part[I.part_off + w] = (red[0] + red[1]) + (red[2] + red[3]);
+  s = block_sum(s, red);
+  double* out = part + (I.part_off + w) * (MOM ? 3 : 1);
+  if constexpr (MOM) {
+    gm = block_sum(gm, red);
+    mm = block_sum(mm, red);
+    if (threadIdx.x == 0) {
+      out[1] = gm;
+      out[2] = mm;
+    }
+  }
+  if (threadIdx.x == 0) out[0] = s;
+}
+
+// |g|^2 of all parameters, in a fixed order
+__global__ __launch_bounds__(256) void k_muon_sqnorm(const double* __restrict__ part, int n, const double* __restrict__ others,
+                                                     int n_others, float* __restrict__ out) {
+  __shared__ double red[4];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256) s += part[3 * (size_t)i];
+  for (int i = threadIdx.x; i < n_others; i += 256) s += others[i];
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) *out = (float)s;
 }
 
 // X0 = G / (|G|_F + eps) as hi + lo, transposed where the matrix is tall, zero in the padding.  One 64 x 64 tile of X: a wave
@@ -236,65 +289,95 @@ __global__ __launch_bounds__(256) void k_orth_init(const Item* __restrict__ item
   const Bufs B = bufs_of(I, ws, b);
   const T* g = MOM ? nullptr : (const T*)I.src + (int64_t)b * I.bs_src;
   const float* gm = MOM ? mo.g_ptrs[I.index] : nullptr;
-  const float* m = MOM ? mo.m + I.flat_off : nullptr;
+  float* m = MOM ? mo.m + I.flat_off : nullptr;
   const float clip = MOM ? clip_of(mo) : 1.f;
   const int64_t ld = MOM ? I.cols : I.ld_src;
-  // columns c .. c + 3 of G's row r, zero behind its edges
-  auto four = [&](int r, int c, float (&v)[4]) {
-    typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    typedef float fvec __attribute__((ext_vector_type(4), aligned(4)));
+  // columns c .. c + 3 of row r of a matrix in G's layout, zero behind its edges
+  auto four = [&](const auto* from, int r, int c, float (&v)[4]) {
+    typedef std::remove_cv_t<std::remove_pointer_t<decltype(from)>> E;
+    typedef E vec __attribute__((ext_vector_type(4), aligned(sizeof(E))));
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = 0.f;
     if (r >= I.rows || c >= I.cols) return;
-    const int64_t at = (int64_t)r * ld + c;
+    const E* at = from + (int64_t)r * ld + c;
     if (c + 3 < I.cols) {
-      if constexpr (MOM) {
-        const fvec a = *reinterpret_cast<const fvec*>(gm + at), o = *reinterpret_cast<const fvec*>(m + at);
+      const vec a = *reinterpret_cast<const vec*>(at);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = update_of(mo, o[e], a[e] * clip);
-      } else {
-        const vec a = *reinterpret_cast<const vec*>(g + at);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (float)a[e];
-      }
+      for (int e = 0; e < 4; ++e) v[e] = (float)a[e];
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (c + e < I.cols) v[e] = MOM ? update_of(mo, m[at + e], gm[at + e] * clip) : (float)g[at + e];
+        if (c + e < I.cols) v[e] = (float)at[e];
     }
   };
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, lg = lane >> 4;
   const bool tall = I.tall;
   const int ti = i0 + wave * 16;  // this wave's 16 rows of the tile, two pairs of column tiles
-  float v[2][2][4];
-  if (tall) {
-    float u[4][4];
+  // the four places of G that this thread reads: where they go in X, or 16 rows apart where the tile is transposed later
+  float v[4][4], old[MOM ? 4 : 1][4];
+  int gr[4], gc[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) four(j0 + k * 16 + (tid >> 4), i0 + (tid & 15) * 4, u[k]);
+  for (int k = 0; k < 4; ++k) {
+    gr[k] = tall ? j0 + k * 16 + (tid >> 4) : ti + l15;
+    gc[k] = tall ? i0 + (tid & 15) * 4 : j0 + k * 16 + 4 * lg;
+    if constexpr (MOM) {
+      four(gm, gr[k], gc[k], v[k]);
+      four((const float*)m, gr[k], gc[k], old[k]);
+    } else {
+      four(g, gr[k], gc[k], v[k]);
+    }
+  }
+  if constexpr (MOM) {  // the tiles of X cover every element once: m moves on here
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      typedef float fvec __attribute__((ext_vector_type(4), aligned(4)));
+      fvec o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = v[k][e] * clip;
+        o[e] = new_m(mo, old[k][e], a);
+        v[k][e] = update_of(mo, o[e], a);
+      }
+      if (gr[k] >= I.rows || gc[k] >= I.cols) continue;
+      float* at = m + (int64_t)gr[k] * ld + gc[k];
+      if (gc[k] + 3 < I.cols) *reinterpret_cast<fvec*>(at) = o;
+      else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (gc[k] + e < I.cols) at[e] = o[e];
+      }
+    }
+  }
+  if (tall) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) tile[(tid & 15) * 4 + e][k * 16 + (tid >> 4)] = u[k][e];
-  } else {
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) four(ti + l15, j0 + q * 32 + h * 16 + 4 * lg, v[q][h]);
+      for (int e = 0; e < 4; ++e) tile[(tid & 15) * 4 + e][k * 16 + (tid >> 4)] = v[k][e];
   }
-  double s = 0.0;
-  for (int i = tid; i < I.parts; i += 256) s += part[I.part_off + (int64_t)b * I.parts + i];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if (lane == 0) red[wave] = s;
-  __syncthreads();
-  const double inv = (double)SX / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + eps);
+  const double* mine = part + (I.part_off + (int64_t)b * I.parts) * (MOM ? 3 : 1);
+  double s = 0.0, gx = 0.0, mx = 0.0;
+  for (int i = tid; i < I.parts; i += 256) {
+    s += mine[i * (MOM ? 3 : 1)];
+    if constexpr (MOM) {
+      gx += mine[i * 3 + 1];
+      mx += mine[i * 3 + 2];
+    }
+  }
+  s = block_sum(s, red);
+  if constexpr (MOM) {
+    gx = block_sum(gx, red);
+    mx = block_sum(mx, red);
+    // u = ca m + cb g of the old m
+    const double mu = mo.mu, ca = mo.nesterov ? mu * mu : mu, cb = (mo.nesterov ? (1.0 - mu) * (1.0 + mu) : 1.0 - mu) * clip;
+    s = ca * ca * mx + 2.0 * ca * cb * gx + cb * cb * s;
+    s = s < 0.0 ? 0.0 : s;  // a NaN stays
+  }
+  const double inv = (double)SX / (sqrt(s) + eps);
   if (tall) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[q][h][e] = tile[wave * 16 + l15][q * 32 + h * 16 + 4 * lg + e];
+      for (int e = 0; e < 4; ++e) v[k][e] = tile[wave * 16 + l15][k * 16 + 4 * lg + e];
   }
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
@@ -306,7 +389,7 @@ __global__ __launch_bounds__(256) void k_orth_init(const Item* __restrict__ item
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x = (float)((double)v[q][k][e] * inv);
+        const float x = (float)((double)v[2 * q + k][e] * inv);
         h[k][e] = (f16)x;
         lv[4 * k + e] = (f16)(x - (float)h[k][e]);
       }
@@ -335,15 +418,23 @@ __device__ __forceinline__ int b_perm(int k) { return (k & ~31) + 8 * ((k & 15) 
 // rows spread over the banks.  LDS-DMA writes lanes in order, so the permutation is made on the global side.
 __device__ __forceinline__ int nt_chunk(int row, int ch) { return ch ^ (row & 7); }
 
-// A (GRAM) or B (!GRAM): T x T tile of a symmetric product P P' of one operand with contiguous contraction, T = 32 WT,
-// 4 waves of 16 WT x 16 WT.  64-deep tiles of both row panels (whole 128-byte lines) go to LDS by LDS-DMA, NB stages.
+// A or B: T x T tile of a symmetric product P P' of one operand with contiguous contraction, T = 32 WT, 4 waves of
+// 16 WT x 16 WT.  64-deep tiles of both row panels (whole 128-byte lines) go to LDS by LDS-DMA, NB stages.  What bounds it is
+// the stream from L2 into LDS, about 14 TB/s: 32 flop per byte at T = 64 (460 TFLOP/s measured), 64 at T = 128.
+// PART / JOIN: few tiles of a long contraction.  PART: workgroup (slice, tile) writes its accumulators as they lie; JOIN adds
+// a tile's slices in order and goes on as GRAM does.
+enum { GRAM = 0, POLY, PART, JOIN };
 constexpr int SYM_TILE = 64;
-template <bool GRAM, int WT, int NB>
+template <int KIND, int WT, int NB>
 __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ items, const int32_t* __restrict__ ends,
-                                                     int count, int cur, char* __restrict__ ws) {
+                                                     int count, int cur, int slices, float* __restrict__ parts,
+                                                     char* __restrict__ ws) {
   constexpr int T = 32 * WT, OP = T * 64, STAGE = 2 * OP, PER = T / 32;
-  __shared__ __attribute__((aligned(1024))) f16 sm[NB * STAGE];
-  const int bid = xcd_remap(blockIdx.x, gridDim.x);
+  __shared__ __attribute__((aligned(1024))) f16 sm[KIND == JOIN ? 8 : NB * STAGE];
+  constexpr int IW = KIND == JOIN ? 1 : WT;  // JOIN: WT workgroups a tile, each with one row of every wave's accumulators
+  const int tiles = KIND == PART ? gridDim.x / slices : gridDim.x / (KIND == JOIN ? WT : 1);
+  const int wg = xcd_remap(blockIdx.x, gridDim.x), slice = KIND == PART ? wg / tiles : 0;
+  const int bid = KIND == JOIN ? wg / WT : wg - slice * tiles, i_of = KIND == JOIN ? wg - bid * WT : 0;
   int first;
   const int it = find_item(ends, count, bid, first);
   const Item& I = items[it];
@@ -356,69 +447,88 @@ __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ it
   while (ti * (ti + 1) / 2 > t) --ti;
   const int tj = t - ti * (ti + 1) / 2;
   const Bufs B = bufs_of(I, ws, b);
-  const f16* src = GRAM ? B.hi(cur) : B.A;
-  const int ld = GRAM ? I.np : mp, K = ld;
+  const f16* src = KIND == POLY ? B.A : B.hi(cur);
+  const int ld = KIND == POLY ? mp : I.np;
+  // this workgroup's share of the contraction, in 64-deep tiles
+  const int nk_all = (ld + 63) / 64, k0 = KIND == PART ? (int)((int64_t)nk_all * slice / slices) : 0;
+  const int k1 = KIND == PART ? (int)((int64_t)nk_all * (slice + 1) / slices) : nk_all;
+  float* part = parts + ((size_t)slice * tiles + bid) * (T * T) + threadIdx.x * 4;
   const int p0 = ti * T, q0 = tj * T;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wp = wave >> 1, wq = wave & 1, l15 = lane & 15, lg = lane >> 4;
-  const f16 *gp[PER], *gq[PER];
-  int gc[PER];
-  unsigned dst[PER];
+  f32x4 acc[IW][WT];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int j = wave + 4 * i, row = 8 * j + (lane >> 3);
-    gc[i] = nt_chunk(row, lane & 7) * 8;
-    gp[i] = src + (size_t)min(p0 + row, mp - 1) * ld;
-    gq[i] = src + (size_t)min(q0 + row, mp - 1) * ld;
-    dst[i] = j * 1024;
-  }
-  const unsigned base = lds_addr(sm);
-  auto issue = [&](int kt, int buf) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int c = min(kt * 64 + gc[i], ld - 8);  // the last tile may be 32 deep: its second half is not multiplied
-      lds_dma16(gp[i] + c, base + buf * (STAGE * 2) + dst[i]);
-      lds_dma16(gq[i] + c, base + buf * (STAGE * 2) + OP * 2 + dst[i]);
-    }
-  };
-  f32x4 acc[WT][WT];
-#pragma unroll
-  for (int i = 0; i < WT; ++i)
+  for (int i = 0; i < IW; ++i)
 #pragma unroll
     for (int j = 0; j < WT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  int fp[WT], fq[WT];
+  if constexpr (KIND != JOIN) {
+    const f16 *gp[PER], *gq[PER];
+    int gc[PER];
+    unsigned dst[PER];
 #pragma unroll
-  for (int i = 0; i < WT; ++i) {  // rows 16 apart share their swizzle: 32 slots further is the chunk with bit 2 flipped
-    const int rp = (wp * WT + i) * 16 + l15, rq = (wq * WT + i) * 16 + l15;
-    fp[i] = rp * 64 + nt_chunk(rp, lg) * 8;
-    fq[i] = OP + rq * 64 + nt_chunk(rq, lg) * 8;
-  }
-  const int nk = (K + 63) / 64;
+    for (int i = 0; i < PER; ++i) {
+      const int j = wave + 4 * i, row = 8 * j + (lane >> 3);
+      gc[i] = nt_chunk(row, lane & 7) * 8;
+      gp[i] = src + (size_t)min(p0 + row, mp - 1) * ld;
+      gq[i] = src + (size_t)min(q0 + row, mp - 1) * ld;
+      dst[i] = j * 1024;
+    }
+    const unsigned base = lds_addr(sm);
+    auto issue = [&](int kt, int buf) {
 #pragma unroll
-  for (int st = 0; st < NB - 1; ++st)
-    if (st < nk) issue(st, st);
-  int buf = 0;
-  for (int kt = 0; kt < nk; ++kt) {
-    wait_stage<2 * PER, NB>(min(nk - 1 - kt, NB - 2));
-    __syncthreads();
-    if (kt + NB - 1 < nk) issue(kt + NB - 1, buf == 0 ? NB - 1 : buf - 1);
-    const f16* s = sm + buf * STAGE;
-    auto half = [&](int x) {
-      f16x8 vp[WT], vq[WT];
-#pragma unroll
-      for (int i = 0; i < WT; ++i) {
-        vp[i] = *reinterpret_cast<const f16x8*>(s + (fp[i] ^ x));
-        vq[i] = *reinterpret_cast<const f16x8*>(s + (fq[i] ^ x));
+      for (int i = 0; i < PER; ++i) {
+        const int c = min((k0 + kt) * 64 + gc[i], ld - 8);  // the last tile may be 32 deep: its second half is not multiplied
+        lds_dma16(gp[i] + c, base + buf * (STAGE * 2) + dst[i]);
+        lds_dma16(gq[i] + c, base + buf * (STAGE * 2) + OP * 2 + dst[i]);
       }
-#pragma unroll
-      for (int i = 0; i < WT; ++i)
-#pragma unroll
-        for (int j = 0; j < WT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vp[i], vq[j], acc[i][j], 0, 0, 0);
     };
-    half(0);
-    if (kt * 64 + 32 < K) half(32);
-    buf = buf == NB - 1 ? 0 : buf + 1;
+    int fp[WT], fq[WT];
+#pragma unroll
+    for (int i = 0; i < WT; ++i) {  // rows 16 apart share their swizzle: 32 slots further is the chunk with bit 2 flipped
+      const int rp = (wp * WT + i) * 16 + l15, rq = (wq * WT + i) * 16 + l15;
+      fp[i] = rp * 64 + nt_chunk(rp, lg) * 8;
+      fq[i] = OP + rq * 64 + nt_chunk(rq, lg) * 8;
+    }
+    const int nk = k1 - k0;
+#pragma unroll
+    for (int st = 0; st < NB - 1; ++st)
+      if (st < nk) issue(st, st);
+    int buf = 0;
+    for (int kt = 0; kt < nk; ++kt) {
+      wait_stage<2 * PER, NB>(min(nk - 1 - kt, NB - 2));
+      __syncthreads();
+      if (kt + NB - 1 < nk) issue(kt + NB - 1, buf == 0 ? NB - 1 : buf - 1);
+      const f16* s = sm + buf * STAGE;
+      auto half = [&](int x) {
+        f16x8 vp[WT], vq[WT];
+#pragma unroll
+        for (int i = 0; i < WT; ++i) {
+          vp[i] = *reinterpret_cast<const f16x8*>(s + (fp[i] ^ x));
+          vq[i] = *reinterpret_cast<const f16x8*>(s + (fq[i] ^ x));
+        }
+#pragma unroll
+        for (int i = 0; i < WT; ++i)
+#pragma unroll
+          for (int j = 0; j < WT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vp[i], vq[j], acc[i][j], 0, 0, 0);
+      };
+      half(0);
+      if ((k0 + kt) * 64 + 32 < ld) half(32);
+      buf = buf == NB - 1 ? 0 : buf + 1;
+    }
+  } else {
+#pragma unroll 2
+    for (int k = 0; k < slices; ++k)
+#pragma unroll
+      for (int j = 0; j < WT; ++j)
+        acc[0][j] += *reinterpret_cast<const f32x4*>(part + (size_t)k * tiles * (T * T) + (i_of * WT + j) * 1024);
+  }
+  if constexpr (KIND == PART) {
+#pragma unroll
+    for (int i = 0; i < WT; ++i)
+#pragma unroll
+      for (int j = 0; j < WT; ++j) *reinterpret_cast<f32x4*>(part + (i * WT + j) * 1024) = acc[i][j];
+    return;
   }
 
   // lane: column q, rows p .. p + 3 of the product
@@ -426,13 +536,13 @@ __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ it
   for (int j = 0; j < WT; ++j) {
     const int q = q0 + (wq * WT + j) * 16 + l15;
     if (q >= mp) continue;
-    const float dq = GRAM ? 0.f : B.dA[q];
+    const float dq = KIND == POLY ? B.dA[q] : 0.f;
 #pragma unroll
-    for (int i = 0; i < WT; ++i) {
-      const int p = p0 + (wp * WT + i) * 16 + 4 * lg;
+    for (int i = 0; i < IW; ++i) {
+      const int p = p0 + (wp * WT + i + i_of) * 16 + 4 * lg;
       if (p >= mp) continue;
       f16x4 h;
-      if constexpr (GRAM) {
+      if constexpr (KIND != POLY) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           h[r] = (f16)(acc[i][j][r] * (SA / (SX * SX)));
@@ -1080,48 +1190,14 @@ __global__ __launch_bounds__(512, 1) void k_orth_small(const Item* __restrict__ 
   }
 }
 
-// sum of squares of all gradients in a fixed order: fp64 partial sums per workgroup, then one workgroup
-__global__ __launch_bounds__(256) void k_sqnorm_parts(const float* const* __restrict__ g_ptrs,
-                                                      const int32_t* __restrict__ numel,
-                                                      const int32_t* __restrict__ chunk_tensor,
-                                                      const int32_t* __restrict__ chunk_off, int n_chunks, int chunk,
-                                                      double* __restrict__ part) {
-  __shared__ double red[4];
-  double s = 0.0;
-  for (int c = blockIdx.x; c < n_chunks; c += gridDim.x) {
-    const int t = chunk_tensor[c], off = chunk_off[c], n = min(chunk, numel[t] - off);
-    const float* g = g_ptrs[t] + off;
-    typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
-    const int n4 = n & ~3;
-    for (int i = 4 * threadIdx.x; i < n4; i += 1024) {
-      const vec v = *reinterpret_cast<const vec*>(g + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s += (double)v[e] * (double)v[e];
-    }
-    for (int i = n4 + threadIdx.x; i < n; i += 256) s += (double)g[i] * (double)g[i];
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
-}
-__global__ __launch_bounds__(256) void k_sqnorm_total(const double* __restrict__ part, int n, float* __restrict__ out) {
-  __shared__ double red[4];
-  double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) s += part[i];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) *out = (float)((red[0] + red[1]) + (red[2] + red[3]));
-}
-constexpr int SQNORM_BLOCKS = 1024;
+constexpr int OTHER_BLOCKS = 256;
 
 // ---- host ----------------------------------------------------------------------------------------------------------
 // What a call over a list of shapes needs; the same arithmetic sizes the workspace, fills the table and sizes the grids
 struct Plan {
-  int count = 0, wt_full = 2;  // tile side of the X product / 32
+  int count = 0, wt_full = 2, wt_gram = 2;  // tile sides of the X product and of A, / 32
+  int slices = 1;                           // of A's contraction
+  int max_np = 0;
   int small_lds = 0;
   bool all_small = true, use_small = true;
   int64_t grid[PREFIXES] = {};
@@ -1165,16 +1241,31 @@ bool plan_item(Plan& P, int32_t rows, int32_t cols, int32_t batch, bool mom, Ite
   if (I) *I = i;
   return true;
 }
-void plan_grids(const Item& i, int wt_full, bool mom, int64_t* g) {
-  const int64_t nt = cdiv64(i.mp, SYM_TILE), b = i.batch, full = b * cdiv64(i.mp, 32 * wt_full) * cdiv64(i.np, 32 * wt_full);
+void plan_grids(const Item& i, int wt_gram, int wt_full, bool mom, int64_t* g) {
+  const int64_t nt = cdiv64(i.mp, SYM_TILE), ng = cdiv64(i.mp, 32 * wt_gram), b = i.batch, full = b * cdiv64(i.mp, 32 * wt_full) * cdiv64(i.np, 32 * wt_full);
   if (i.small) g[P_SMALL] += b;
   if (i.small && !mom) return;  // reads G and writes O by itself
   g[P_NORM] += b * i.parts;
   g[P_INIT] += b * cdiv64(i.mp, INIT_TILE) * cdiv64(i.np, INIT_TILE);
   g[P_LAST] += full;
   if (i.small) return;
-  g[P_SYM] += b * (nt * (nt + 1) / 2);
+  g[P_GRAM] += b * (ng * (ng + 1) / 2);
+  g[P_POLY] += b * (nt * (nt + 1) / 2);
   g[P_FULL] += full;
+}
+
+// A of long matrices (a contraction of 2048 and more): 128-wide tiles where they are many, the contraction cut into slices of
+// at least 512 until about 512 workgroups share the work.  Measured, slices and 64-wide tiles against the uncut form:
+void plan_slices(Plan& P) {  // grid[P_GRAM] holds 128-wide tiles
+  P.wt_gram = 2;
+  P.slices = 1;
+  if (P.max_np < 2048 || P.grid[P_GRAM] == 0) return;
+  int64_t tiles = P.grid[P_GRAM];
+  if (tiles >= 100 && P.max_np >= 4096) P.wt_gram = 4;
+  else tiles *= 4;  // about as many 64-wide ones
+  const int64_t most = P.max_np / 512, want = 512 / tiles;
+  P.slices = (int)(want < most ? want : most);
+  if (P.slices <= 1) { P.slices = 1; P.wt_gram = 2; }
 }
 
 // plan buffer (device): Item[count], int32 ends[PREFIXES][count], then the fp64 partial sums
@@ -1184,18 +1275,20 @@ template <class F>
 bool make_plan(int32_t count, bool mom, F shape, Plan& P) {  // shape(i, rows, cols, batch)
   if (count < 0) return false;
   for (int pass = 0; pass < 2; ++pass) {
-    P.parts = 0; P.bytes = 0; P.flops = 0; P.count = 0; P.small_lds = 0;
+    P.parts = 0; P.bytes = 0; P.flops = 0; P.count = 0; P.small_lds = 0; P.max_np = 0;
     for (int k = 0; k < PREFIXES; ++k) P.grid[k] = 0;
     for (int32_t i = 0; i < count; ++i) {
       int32_t r, c, b;
       shape(i, r, c, b);
       Item it;
       if (!plan_item(P, r, c, b, mom, &it)) return false;
-      plan_grids(it, pass == 0 ? 4 : P.wt_full, mom, P.grid);
+      plan_grids(it, pass == 0 ? 4 : P.wt_gram, pass == 0 ? 4 : P.wt_full, mom, P.grid);
+      if (it.batch && !it.small && it.np > P.max_np) P.max_np = it.np;
     }
     if (pass == 0) {
       P.use_small = P.all_small;
       P.wt_full = P.grid[P_LAST] >= 384 ? 4 : 2;
+      plan_slices(P);
     }
   }
   for (int k = 0; k < PREFIXES; ++k)
@@ -1215,7 +1308,7 @@ int write_table(int32_t count, const Plan& P, bool mom, F fill, void* table, hip
     const int n = count - first < TABLE_BATCH ? count - first : TABLE_BATCH;
     for (int k = 0; k < n; ++k) {
       fill(first + k, run, eb.e[k].item);
-      plan_grids(eb.e[k].item, P.wt_full, mom, g);
+      plan_grids(eb.e[k].item, P.wt_gram, P.wt_full, mom, g);
       for (int q = 0; q < PREFIXES; ++q) eb.e[k].end[q] = (int32_t)g[q];
     }
     hipLaunchKernelGGL(k_orth_table, dim3(1), dim3(64), 0, s, eb, first, n, count, items, ends);
@@ -1228,21 +1321,32 @@ struct Ptrs {
   const Item* items;
   const int32_t* ends;
   double* part;
+  float* slices;
   char* ws;
   int count;
   const int32_t* end(int k) const { return ends + (size_t)k * count; }
 };
-size_t ws_bytes_of(const Plan& P) { return align256((size_t)P.parts * 8) + P.bytes + 256; }
+size_t slice_bytes(const Plan& P) {  // partial tiles of A
+  return P.slices == 1 ? 0 : (size_t)P.grid[P_GRAM] * P.slices * (size_t)(32 * P.wt_gram) * (32 * P.wt_gram) * 4;
+}
+size_t part_bytes(const Plan& P) { return align256(((size_t)P.parts * 3 + OTHER_BLOCKS) * 8); }
+size_t ws_bytes_of(const Plan& P) { return part_bytes(P) + slice_bytes(P) + P.bytes; }
 Ptrs ptrs_of(int count, const Plan& P, const void* table, void* ws) {
   Ptrs r;
   r.items = (const Item*)table;
   r.ends = (const int32_t*)((const char*)table + align256((size_t)count * sizeof(Item)));
   r.part = (double*)ws;
-  r.ws = (char*)ws + align256((size_t)P.parts * 8);
+  r.slices = (float*)((char*)ws + part_bytes(P));
+  r.ws = (char*)r.slices + slice_bytes(P);
   r.count = count;
   return r;
 }
 
+template <int KIND, int WT, int NB>
+void sym(const Plan& P, const Ptrs& p, int g, int cur, hipStream_t s) {
+  hipLaunchKernelGGL((k_orth_sym<KIND, WT, NB>), dim3((unsigned)(P.grid[g] * (KIND == PART ? P.slices : KIND == JOIN ? WT : 1))), dim3(256), 0, s,
+                     p.items, p.end(g), p.count, cur, P.slices, p.slices, p.ws);
+}
 template <int MODE, int WT, int NB>
 void apply(const Plan& P, const Ptrs& p, int cur, int otype, const Momentum& mo, hipStream_t s) {
   constexpr int G = MODE == MID ? P_FULL : P_LAST;
@@ -1251,12 +1355,13 @@ void apply(const Plan& P, const Ptrs& p, int cur, int otype, const Momentum& mo,
 }
 template <int MODE>
 int run_steps(const Plan& P, const Ptrs& p, int steps, int otype, const Momentum& mo, hipStream_t s) {
-  const dim3 gs((unsigned)P.grid[P_SYM]);
   const bool only_last = P.grid[P_FULL] == 0;  // small matrices alone: their steps are made
   for (int k = only_last ? steps - 1 : 0, cur = 0; k < steps; ++k, cur ^= 1) {
     if (!only_last) {
-      hipLaunchKernelGGL((k_orth_sym<true, 2, 2>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
-      hipLaunchKernelGGL((k_orth_sym<false, 2, 2>), gs, dim3(256), 0, s, p.items, p.end(P_SYM), p.count, cur, p.ws);
+      if (P.slices == 1) sym<GRAM, 2, 2>(P, p, P_GRAM, cur, s);
+      else if (P.wt_gram == 4) { sym<PART, 4, 2>(P, p, P_GRAM, cur, s); sym<JOIN, 4, 2>(P, p, P_GRAM, cur, s); }
+      else { sym<PART, 2, 2>(P, p, P_GRAM, cur, s); sym<JOIN, 2, 2>(P, p, P_GRAM, cur, s); }
+      sym<POLY, 2, 2>(P, p, P_POLY, cur, s);
     }
     if (k + 1 < steps) {
       if (P.wt_full == 4) apply<MID, 4, 2>(P, p, cur, otype, mo, s);
@@ -1271,10 +1376,14 @@ int run_steps(const Plan& P, const Ptrs& p, int steps, int otype, const Momentum
 }
 
 template <class T, bool MOM>
-int run_all(const Plan& P, const Ptrs& p, int steps, int otype, float eps, const Momentum& mo, hipStream_t s) {
+int run_all(const Plan& P, const Ptrs& p, int steps, int otype, float eps, const Momentum& mo, hipStream_t s,
+            float* sqnorm = nullptr) {
   if (P.grid[P_NORM]) {
-    hipLaunchKernelGGL((k_orth_norm<T, MOM>), dim3((unsigned)P.grid[P_NORM]), dim3(256), 0, s, p.items, p.end(P_NORM), p.count,
+    const int blocks = (int)P.grid[P_NORM], extra = mo.n_chunks < OTHER_BLOCKS ? mo.n_chunks : OTHER_BLOCKS;
+    hipLaunchKernelGGL((k_orth_norm<T, MOM>), dim3(blocks + extra), dim3(256), 0, s, p.items, p.end(P_NORM), p.count, blocks,
                        p.part, mo);
+    if (MOM && mo.sqnorm)
+      hipLaunchKernelGGL(k_muon_sqnorm, dim3(1), dim3(256), 0, s, p.part, blocks, mo.others, extra, sqnorm);
     hipLaunchKernelGGL((k_orth_init<T, MOM>), dim3((unsigned)P.grid[P_INIT]), dim3(256), 0, s, p.items, p.end(P_INIT), p.count,
                        p.part, (double)eps, p.ws, mo);
     SWG_LAUNCH_CHECK();
@@ -1362,40 +1471,31 @@ int swg_muon_table(int32_t count, const swg_muon_item* items, void* table, size_
 }
 
 int swg_muon_ema_step(int32_t count, const swg_muon_item* items, const void* table, const void* p_ptrs, const void* g_ptrs,
-                      float* m, float* ema, int64_t total, int32_t n_ema, const float* ema_decay, const float* sqnorm,
-                      float max_norm, float lr, float momentum, int32_t nesterov, float weight_decay, int32_t steps,
-                      float eps, void* ws, size_t ws_bytes, void* stream) {
-  if (count <= 0 || total <= 0 || n_ema < 0 || n_ema > 8 || steps < 1 || steps > 64 || !(eps >= 0.f)) return SWG_E_SHAPE;
+                      float* m, float* ema, int64_t total, int32_t n_ema, const float* ema_decay, const int32_t* numel,
+                      const int32_t* chunk_tensor, const int32_t* chunk_off, int32_t n_chunks, float* sqnorm, float max_norm,
+                      float lr, float momentum, int32_t nesterov, float weight_decay, int32_t steps, float eps, void* ws,
+                      size_t ws_bytes, void* stream) {
+  if (count <= 0 || total <= 0 || n_ema < 0 || n_ema > 8 || steps < 1 || steps > 64 || n_chunks < 0 || !(eps >= 0.f))
+    return SWG_E_SHAPE;
   if (!items || !table || !p_ptrs || !g_ptrs || !m || !ws || (n_ema > 0 && (!ema || !ema_decay))) return SWG_E_NULL;
+  if (sqnorm && n_chunks > 0 && (!numel || !chunk_tensor || !chunk_off)) return SWG_E_NULL;
   Plan P;
   if (!muon_plan(count, items, P)) return SWG_E_SHAPE;
   if (ws_bytes < ws_bytes_of(P)) return SWG_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
+  const Ptrs p = ptrs_of(count, P, table, ws);
   Momentum mo = {};
   mo.g_ptrs = (const float* const*)g_ptrs; mo.p_ptrs = (float* const*)p_ptrs;
   mo.m = m; mo.ema = ema; mo.total = total; mo.sqnorm = sqnorm; mo.max_norm = max_norm; mo.mu = momentum; mo.lr = lr;
   mo.keep = 1.f - lr * weight_decay; mo.nesterov = nesterov; mo.n_ema = n_ema;
   for (int k = 0; k < n_ema; ++k) mo.ema_w[k] = 1.0f - ema_decay[k];
+  if (sqnorm) {
+    mo.numel = numel; mo.chunk_tensor = chunk_tensor; mo.chunk_off = chunk_off; mo.n_chunks = n_chunks;
+    mo.chunk = swg_optim_chunk();
+    mo.others = p.part + (size_t)P.parts * 3;
+  }
   SwgProfScope ps(KID_ORTH, P.flops * steps, 0.0, s);
-  const Ptrs p = ptrs_of(count, P, table, ws);
-  return run_all<float, true>(P, p, steps, 0, eps, mo, s);
-}
-
-size_t swg_grad_sqnorm_ordered_workspace_bytes(void) { return SQNORM_BLOCKS * sizeof(double); }
-
-int swg_grad_sqnorm_ordered(const void* g_ptrs, const int32_t* numel, const int32_t* chunk_tensor, const int32_t* chunk_off,
-                            int32_t n_chunks, float* sqnorm, void* ws, size_t ws_bytes, void* stream) {
-  if (!g_ptrs || !numel || !chunk_tensor || !chunk_off || !sqnorm || !ws) return SWG_E_NULL;
-  if (n_chunks <= 0) return SWG_E_SHAPE;
-  if (ws_bytes < SQNORM_BLOCKS * sizeof(double)) return SWG_E_WORKSPACE;
-  hipStream_t s = (hipStream_t)stream;
-  const int grid = n_chunks < SQNORM_BLOCKS ? n_chunks : SQNORM_BLOCKS;
-  SwgProfScope ps(KID_OPTIM, 0.0, 0.0, s);
-  hipLaunchKernelGGL(k_sqnorm_parts, dim3(grid), dim3(256), 0, s, (const float* const*)g_ptrs, numel, chunk_tensor, chunk_off,
-                     n_chunks, swg_optim_chunk(), (double*)ws);
-  hipLaunchKernelGGL(k_sqnorm_total, dim3(1), dim3(256), 0, s, (const double*)ws, grid, sqnorm);
-  SWG_LAUNCH_CHECK();
-  return 0;
+  return run_all<float, true>(P, p, steps, 0, eps, mo, s, sqnorm);
 }
 
 }  // extern "C"

@@ -247,7 +247,6 @@ class FusedMuonEMA(FusedAdamEMA):
             raise L.SwgError("swg_muon_workspace_bytes: unsupported matrix shapes")
         nbytes = int(L.lib.swg_muon_table_bytes(len(matrices)))
         self._table = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        self._sq_ws = torch.empty(int(L.lib.swg_grad_sqnorm_ordered_workspace_bytes()), dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
             L.check(L.lib.swg_muon_table(len(matrices), self._items, self._table.data_ptr(), nbytes, stream_ptr()),
                     "swg_muon_table")
@@ -288,30 +287,26 @@ class FusedMuonEMA(FusedAdamEMA):
         self._point()
         mat, st = self.param_groups[0], stream_ptr()
         tables = (self._p_ptrs.data_ptr(), self._g_ptrs.data_ptr())
-        sq = None
-        if self.max_norm is not None:
-            sq = self._sqnorm.data_ptr()
-            L.check(L.lib.swg_grad_sqnorm_ordered(tables[1], self._numel.data_ptr(), self._ct.data_ptr(), self._co.data_ptr(),
-                                                  self.n_chunks, sq, self._sq_ws.data_ptr(), self._sq_ws.numel(), st),
-                    "swg_grad_sqnorm_ordered")
+        sq = None if self.max_norm is None else self._sqnorm.data_ptr()
         self.step_count += 1
         n_ema = len(self.ema_betas)
         dec = (C.c_float * 8)(*(self._ema_decays() + [0.0] * (8 - n_ema)))
         clip = float(self.max_norm or 0.0)
         ws = workspace(self.m.device, self._ws_bytes)
+        first, n = self._first_other, self.n_chunks - self._first_other
+        chunks = (self._ct.data_ptr() + 4 * first, self._co.data_ptr() + 4 * first, n)  # the other parameters'
         L.check(L.lib.swg_muon_ema_step(self.n_matrices, self._items, self._table.data_ptr(), *tables, self.m.data_ptr(),
-                                        self.ema.data_ptr(), self.total, n_ema, dec, sq, clip, float(mat["lr"]),
-                                        float(mat["momentum"]), int(mat["nesterov"]), float(mat["weight_decay"]),
-                                        int(mat["ns_steps"]), 1e-7, ws.data_ptr(), ws.numel(), st), "swg_muon_ema_step")
-        if len(self.param_groups) > 1:
-            grp, first = self.param_groups[1], self._first_other
+                                        self.ema.data_ptr(), self.total, n_ema, dec, self._numel.data_ptr(), *chunks, sq, clip,
+                                        float(mat["lr"]), float(mat["momentum"]), int(mat["nesterov"]),
+                                        float(mat["weight_decay"]), int(mat["ns_steps"]), 1e-7, ws.data_ptr(), ws.numel(), st),
+                "swg_muon_ema_step")
+        if n:
+            grp = self.param_groups[1]
             b1, b2 = grp["betas"]
-            L.check(L.lib.swg_adam_ema_step(*tables, self._numel.data_ptr(), self._flat_off.data_ptr(),
-                                            self._ct.data_ptr() + 4 * first, self._co.data_ptr() + 4 * first,
-                                            self.n_chunks - first, self.m.data_ptr(), self.v.data_ptr(),
-                                            self.ema.data_ptr(), self.total, n_ema, dec, sq, clip, float(grp["lr"]),
-                                            float(b1), float(b2), float(grp["eps"]), float(grp["weight_decay"]),
-                                            self.step_count, st), "swg_adam_ema_step")
+            L.check(L.lib.swg_adam_ema_step(*tables, self._numel.data_ptr(), self._flat_off.data_ptr(), *chunks,
+                                            self.m.data_ptr(), self.v.data_ptr(), self.ema.data_ptr(), self.total, n_ema, dec,
+                                            sq, clip, float(grp["lr"]), float(b1), float(b2), float(grp["eps"]),
+                                            float(grp["weight_decay"]), self.step_count, st), "swg_adam_ema_step")
         if n_ema:
             self.ema_updates += 1
         self._bump_versions()

@@ -97,6 +97,19 @@ def test_large_tiles():
     _check(h, S.orthogonalise(h))
 
 
+@pytest.mark.parametrize("shape", [(16, 4096), (130, 2500), (2048, 257), (65, 8192), (700, 2049), (2, 300, 2048), (1800, 2300)])
+def test_long_contractions(shape):
+    """A cut along the contraction: slices of uneven length, 64- and 128-wide tiles, batches, both orientations."""
+    import swingnn_amd as S
+    g = _gauss(shape, sum(shape))
+    o = S.orthogonalise(g)
+    for gg, oo in zip(g, o) if g.dim() == 3 else ((g, o),):
+        _check(gg, oo)
+    assert torch.equal(o, S.orthogonalise(g))
+    pair = S.orthogonalise([g, _gauss((200, 40), 3)])    # beside a matrix with a short one
+    _check(_gauss((200, 40), 3), pair[1])
+
+
 def test_lists_of_mixed_shapes():
     import swingnn_amd as S
     shapes = [(3, 40, 96), (96, 96), (0, 5), (2, 300, 64), (64, 0), (0, 7, 7), (1, 1), (130, 260), (513, 33)]
@@ -332,30 +345,32 @@ def test_refused_checkpoints_and_groups():
         opt.step()                              # no gradients
 
 
-def test_ordered_gradient_norm():
-    """swg_grad_sqnorm_ordered against float64: equal to rounding of one float32, the same bits every time, captured too."""
+@pytest.mark.parametrize("n_others", [0, 1, 700])
+def test_gradient_norm(n_others):
+    """grad_norm() against float64: one rounding to float32 of the sum and one of the root, and the same bits every time;
+    more other parameters than workgroups that sum them."""
     import swingnn_amd as S
-    from swingnn_amd import _lib as L, engine as E
-    params, k = _network(6)
-    _grads(params, 3, 1e3)
-    opt = S.FusedMuonEMA(params[:k], params[k:], lr=0.0, max_norm=1.0)
-    opt._point()
-    want = sum(float(p.grad.double().square().sum()) for p in params)
+    mats = [torch.nn.Parameter(_gauss(s, i)) for i, s in enumerate([(96, 96), (3, 5), (300, 257)])]
+    others = [torch.nn.Parameter(_gauss((1 + 37 * k,), k)) for k in range(n_others)]
+    opt = S.FusedMuonEMA(mats, others, lr=0.0, max_norm=1.0)
+    _grads(mats + others, 3, 1e3)
+    want = sum(float(p.grad.double().square().sum()) for p in mats + others) ** 0.5
+    got = []
+    for _ in range(2):
+        opt.step()
+        got.append(float(opt.grad_norm()))
+    assert got[0] == got[1] and abs(got[0] - want) <= 2.0 ** -23 * want
 
-    def call():
-        L.check(L.lib.swg_grad_sqnorm_ordered(opt._g_ptrs.data_ptr(), opt._numel.data_ptr(), opt._ct.data_ptr(), opt._co.data_ptr(),
-                                              opt.n_chunks, opt._sqnorm.data_ptr(), opt._sq_ws.data_ptr(), opt._sq_ws.numel(),
-                                              E.stream_ptr()), "swg_grad_sqnorm_ordered")
-    call()
-    first = float(opt._sqnorm)
-    assert abs(first - want) <= 2.0 ** -23 * want
-    gr = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(gr):
-        call()
-    for _ in range(3):
-        opt._sqnorm.fill_(-1)
-        gr.replay()
-        assert float(opt._sqnorm) == first
+
+def test_update_that_cancels():
+    """g = -a m / b: the update is nothing but rounding, its norm from the three sums is 1e-16 of the terms'."""
+    import swingnn_amd as S
+    p = torch.nn.Parameter(_gauss((64, 200), 1))
+    opt = S.FusedMuonEMA([p], lr=1.0, momentum=0.5)
+    opt.m.copy_(_gauss((64 * 200,), 2))
+    p.grad = -(opt.m.view(64, 200) * (0.25 / 0.75))
+    opt.step()
+    assert bool(p.isfinite().all())
 
 
 def test_training_run_together():

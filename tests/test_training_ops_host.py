@@ -137,9 +137,10 @@ def test_muon_refusals(S):
     assert len(mats) == 1 and mats[0] is lin.weight and len(others) == 6
     items = (L.SwgMuonItem * 1)(L.SwgMuonItem(0, 8, 8, 0, 1.0))
     p, st = 4096, L.lib.swg_muon_ema_step
-    ok = [1, items, p, p, p, p, p, 64, 0, None, None, 0.0, 1e-3, 0.9, 1, 0.0, 5, 1e-7, p, 1 << 20, None]
-    for at, bad, code in ((0, 0, -1), (7, 0, -1), (8, 9, -1), (16, 0, -1), (16, 65, -1), (17, -1.0, -1), (1, None, -4), (2, None, -4), (3, None, -4),
-                          (4, None, -4), (5, None, -4), (18, None, -4), (19, 64, -3), (8, 1, -4)):
+    ok = [1, items, p, p, p, p, p, 64, 0, None, p, p, p, 1, p, 0.0, 1e-3, 0.9, 1, 0.0, 5, 1e-7, p, 1 << 20, None]
+    for at, bad, code in ((0, 0, -1), (7, 0, -1), (8, 9, -1), (13, -1, -1), (20, 0, -1), (20, 65, -1), (21, -1.0, -1), (1, None, -4), (2, None, -4),
+                          (3, None, -4), (4, None, -4), (5, None, -4), (10, None, -4), (11, None, -4), (12, None, -4), (22, None, -4),
+                          (23, 64, -3), (8, 1, -4)):
         args = list(ok)
         args[at] = bad
         assert st(*args) == code, at
@@ -148,6 +149,3 @@ def test_muon_refusals(S):
     assert L.lib.swg_muon_table(1, items, None, 1 << 20, None) == -4
     zero = (L.SwgMuonItem * 1)(L.SwgMuonItem(0, 0, 8, 0, 1.0))
     assert L.lib.swg_muon_table(1, zero, p, 1 << 20, None) == -1
-    n = L.lib.swg_grad_sqnorm_ordered
-    assert n(None, p, p, p, 1, p, p, 8192, None) == -4 and n(p, p, p, p, 0, p, p, 8192, None) == -1
-    assert n(p, p, p, p, 1, p, p, 8, None) == -3
