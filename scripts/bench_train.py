@@ -7,6 +7,7 @@
 --ddp stock : the drop-in module wrapped in torch's DistributedDataParallel, as utils/dist_training.py:67-74 does
 --ddp native: parallel.enable_gradient_sync -- the HIP backward's flat gradient buffer is all-reduced in a few large
               asynchronous RCCL messages while the remaining backward kernels run (no DDP wrapper, no bucket copies)
+--optim muon: FusedMuonEMA (orthogonalised updates of the Linear weights) in place of FusedAdamEMA
 `batch` is the PER-RANK batch (weak scaling: the reference's per-GPU batch is batch_size / world, dataloader.py:27-31).
 Rank 0 prints one JSON line in DDP mode (ms per step = max over ranks, graphs/s = all ranks' graphs / that time).
 SWG_BENCH_REHEARSAL=1: ranks share the visible GPU(s) and meet over gloo (code-path check on a one-GPU box, not a
@@ -27,6 +28,7 @@ ap.add_argument("name", nargs="?", default="com", choices=list(CFG))
 ap.add_argument("batch", nargs="?", type=int, default=None)
 ap.add_argument("steps", nargs="?", type=int, default=10)
 ap.add_argument("--ddp", choices=("stock", "native"), default=None)
+ap.add_argument("--optim", choices=("adam", "muon"), default="adam")
 args = ap.parse_args()
 name, c = args.name, CFG[args.name]
 B = args.batch or c["B"]
@@ -59,7 +61,8 @@ if args.ddp == "stock":
 elif args.ddp == "native":
     from swingnn_amd import parallel
     parallel.enable_gradient_sync(model, min_world=1)
-opt = S.FusedAdamEMA(model.parameters(), lr=1e-4, max_norm=10.0, ema_betas=(0.9, 0.95, 0.99, 0.999, 0.9999))
+opt_kw = dict(lr=1e-4, max_norm=10.0, ema_betas=(0.9, 0.95, 0.99, 0.999, 0.9999))
+opt = S.FusedAdamEMA(model.parameters(), **opt_kw) if args.optim == "adam" else S.FusedMuonEMA(*S.FusedMuonEMA.split(model), **opt_kw)
 obj = S.EDMObjectiveGenerator("edm", "edm", dev=dev)
 loss_fn = S.RainbowLoss(1.0, False, "edm")
 torch.manual_seed(1234 + rank)    # per-rank data and noise (utils/arg_parser.py:254-255)

@@ -78,8 +78,9 @@ __global__ void k_orth_table(EntryBatch b, int first, int count, int total, Item
 
 // Which item workgroup `bid` works on, and the first workgroup of that item: lane l looks at entry l
 __device__ __forceinline__ int find_item(const int32_t* __restrict__ ends, int n, int bid, int& first) {
-  const int lane = threadIdx.x & 63;
   first = 0;
+  if (n == 1) return 0;
+  const int lane = threadIdx.x & 63;
   for (int base = 0;; base += 64) {
     const int e = base + lane < n ? ends[base + lane] : 0x7fffffff;
     const unsigned long long before = __ballot(e <= bid);

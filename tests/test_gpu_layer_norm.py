@@ -17,6 +17,13 @@ U = 2.0 ** -24
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
 
+@pytest.fixture(autouse=True)
+def _grad_mode():
+    """Other modules of the suite switch gradients off for the process."""
+    with torch.enable_grad():
+        yield
+
+
 def _half_step(t):
     return 0.0 if t is F32 else torch.finfo(t).eps / 2
 

@@ -12,6 +12,13 @@ DEV = "cuda:0"
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
 
+@pytest.fixture(autouse=True)
+def _grad_mode():
+    """Other modules of the suite switch gradients off for the process."""
+    with torch.enable_grad():
+        yield
+
+
 def _gauss(shape, seed, t=F32):
     return torch.randn(*shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(seed)).to(t)
 
