@@ -1275,7 +1275,7 @@ size_t table_bytes(int count) { return align256((size_t)count * sizeof(Item)) + 
 template <class F>
 bool make_plan(int32_t count, bool mom, F shape, Plan& P) {  // shape(i, rows, cols, batch)
   if (count < 0) return false;
-  for (int pass = 0; pass < 2; ++pass) {
+  for (int pass = 0; pass < 3; ++pass) {  // is every matrix small?  counts of 128-wide tiles, counts of the tiles chosen
     P.parts = 0; P.bytes = 0; P.flops = 0; P.count = 0; P.small_lds = 0; P.max_np = 0;
     for (int k = 0; k < PREFIXES; ++k) P.grid[k] = 0;
     for (int32_t i = 0; i < count; ++i) {
@@ -1283,11 +1283,11 @@ bool make_plan(int32_t count, bool mom, F shape, Plan& P) {  // shape(i, rows, c
       shape(i, r, c, b);
       Item it;
       if (!plan_item(P, r, c, b, mom, &it)) return false;
-      plan_grids(it, pass == 0 ? 4 : P.wt_gram, pass == 0 ? 4 : P.wt_full, mom, P.grid);
+      plan_grids(it, pass < 2 ? 4 : P.wt_gram, pass < 2 ? 4 : P.wt_full, mom, P.grid);
       if (it.batch && !it.small && it.np > P.max_np) P.max_np = it.np;
     }
-    if (pass == 0) {
-      P.use_small = P.all_small;
+    if (pass == 0) P.use_small = P.all_small;
+    if (pass == 1) {
       P.wt_full = P.grid[P_LAST] >= 384 ? 4 : 2;
       plan_slices(P);
     }

@@ -41,6 +41,7 @@ class FusedAdamEMA(torch.optim.Optimizer):
             raise NotImplementedError("at most 8 EMA copies")
         self.ema_inv_gamma, self.ema_power = float(ema_inv_gamma), float(ema_power)
         self.params = params
+        self._shapes = [p.shape for p in params]
         dev = self.params[0].device
         if dev.type != "cuda":
             raise RuntimeError("swingnn_amd runs on an MI355X only; there is no CPU fallback")
@@ -159,6 +160,9 @@ class FusedAdamEMA(torch.optim.Optimizer):
             self._g_key = key
         pkey = tuple(p.data_ptr() for p in self.params)
         if pkey != self._p_key:  # parameter storage moved (model.to(), p.data = ..., load_state_dict(assign=True))
+            for p, shape in zip(self.params, self._shapes):
+                if p.dtype != torch.float32 or not p.is_contiguous() or p.device != self.m.device or p.shape != shape:
+                    raise NotImplementedError(f"{type(self).__name__}: parameters stay contiguous fp32 of their shape and device")
             self._p_ptrs.copy_(torch.tensor(pkey, dtype=torch.int64), non_blocking=False)
             self._p_key = pkey
             self._views = None
@@ -279,6 +283,8 @@ class FusedMuonEMA(FusedAdamEMA):
     def step(self, closure=None):
         if closure is not None:
             raise NotImplementedError("closure")
+        if torch.cuda.is_current_stream_capturing():
+            raise NotImplementedError("FusedMuonEMA.step in a graph: its step count and EMA decays are host numbers")
         with torch.cuda.device(self.params[0].device):
             self._step()
         return None

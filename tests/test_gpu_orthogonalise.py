@@ -168,6 +168,29 @@ def test_zero_and_non_finite_matrices():
         _check(g[k], o[k])
 
 
+def test_non_finite_matrices_of_the_many_launch_form():
+    import swingnn_amd as S
+    g = _gauss((4, 150, 300), 9)
+    g[1] = 0
+    g[2, 149, 299] = float("inf")
+    o = S.orthogonalise(g)
+    assert not o[1].any() and bool(o[2].isnan().all())
+    for k in (0, 3):
+        _check(g[k], o[k])
+    t = _gauss((2, 2300, 140), 5)               # a contraction in slices
+    t[0, 7, 7] = float("nan")
+    o = S.orthogonalise(t)
+    assert bool(o[0].isnan().all())
+    _check(t[1], o[1])
+
+
+def test_small_ones_beside_a_long_one():
+    import swingnn_amd as S
+    mats = [_gauss((140, 2100), 1)] + [_gauss((30 + k, 50), k) for k in range(40)]
+    for g, o in zip(mats, S.orthogonalise(mats)):
+        _check(g, o)
+
+
 def test_c_entry_leaves_gaps_alone_and_reads_its_strides():
     from swingnn_amd import _lib as L, engine as E
     g = _gauss((3, 50, 80), 4)
@@ -333,6 +356,37 @@ def test_optimizer_without_others_and_moved_storage():
     assert float((p.detach().double() - want).abs().max()) < 1e-2 * 0.2 * 8 * 5e-3
 
 
+@pytest.mark.parametrize("shapes", [[(33, 50), (7,)], [(160, 230), (300, 131), (9,)]])
+def test_parameters_at_odd_addresses(shapes):
+    """Views at 4-byte offsets, as slices of a flat buffer have them; what lies between them stays."""
+    import swingnn_amd as S
+    flat, gflat = torch.full((100000,), 3.0, device=DEV), _gauss((100000,), 1)
+    at, params = 1, []
+    for s in shapes:
+        n = 1
+        for d in s:
+            n *= d
+        flat[at:at + n] = 0.02 * _gauss((n,), n)
+        params.append(torch.nn.Parameter(flat[at:at + n].view(s)))
+        params[-1].grad = gflat[at + 2:at + 2 + n].view(s)
+        at += n + 3
+    before = flat.clone()
+    opt = S.FusedMuonEMA(params[:-1], params[-1:], lr=1e-2, ema_betas=(0.9,))
+    opt.step()
+    torch.cuda.synchronize()
+    at = 1
+    for p in params:
+        n = p.numel()
+        if p.dim() == 2:
+            ref, each, _ = R.bounds(0.05 * 1.95 * p.grad)
+            f = 1e-2 * 0.2 * max(p.shape) ** 0.5
+            want = before[at:at + n].view(p.shape).double() - f * ref
+            assert float((p.detach().double() - want).abs().max()) <= f * each + 1e-7
+        assert torch.equal(flat[at + n:at + n + 3], before[at + n:at + n + 3])
+        at += n + 3
+    assert torch.equal(flat[at:], before[at:])
+
+
 def test_refused_checkpoints_and_groups():
     import swingnn_amd as S
     params, k = _network(5)
@@ -350,6 +404,21 @@ def test_refused_checkpoints_and_groups():
         opt.step(lambda: None)
     with pytest.raises(RuntimeError):
         opt.step()                              # no gradients
+    _grads(params, 1)
+    params[1].data = params[1].data.t().contiguous().t()
+    with pytest.raises(NotImplementedError):
+        opt.step()                              # rows and columns exchanged in memory
+    params[1].data = params[1].data.contiguous()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        with pytest.raises(NotImplementedError):
+            opt.step()
+        graph.capture_end()
+    torch.cuda.current_stream().wait_stream(side)
+    opt.step()
 
 
 @pytest.mark.parametrize("n_others", [0, 1, 700])
