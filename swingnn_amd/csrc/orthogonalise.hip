@@ -15,8 +15,15 @@
 // fp16 off-diagonals.  Together: 4e-5 ... 1.5e-3 of |O| for every spectrum tried (bf16 operands: up to 1.5e-2).
 //
 // Every matrix of a call goes through the same launches: one to sum |G|^2 in parts (fp64), one to write X0, three per
-// step (A, B, X).  A workgroup finds its matrix in a table of running tile counts (one load per lane and a ballot).
-// A and B are symmetric: the tiles on and below the diagonal are computed and written twice.
+// step (A, B, X; four where A's contraction is cut).  A workgroup finds its matrix in a table of running tile counts (one
+// load per lane and a ballot).  A and B are symmetric: the tiles on and below the diagonal are computed and written twice.
+// A call of small matrices alone takes one workgroup per matrix for all steps (k_orth_small).
+//
+// Measured, five steps on the GPU (fp32 G, a large library product in fp16 reaches 1107 TFLOP/s, a large copy 4.9 TB/s):
+// 48 matrices of 384-channel blocks 470 us, 2048 x 8192 (bf16 G) 875 us = 640 TFLOP/s of the 558 GFLOP that the symmetric
+// halves need, 96 x 96 30 us.  Bounds: A and B the stream from L2 into LDS (with the products taken out 21 of 25 us
+// remain); X at K = 384 its own reads and writes (hi, lo in; hi, lo out: 8 bytes an element, 5.4 TB/s), at K = 2048 the
+// same stream (66 of 88 us); below about 300 rows the launches, 4 to 6 us each.
 #include "common.h"
 #include <type_traits>
 
@@ -455,6 +462,7 @@ __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ it
   const int k1 = KIND == PART ? (int)((int64_t)nk_all * (slice + 1) / slices) : nk_all;
   float* part = parts + ((size_t)slice * tiles + bid) * (T * T) + threadIdx.x * 4;
   const int p0 = ti * T, q0 = tj * T;
+  const bool diag = ti == tj;  // both panels are the same one
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wp = wave >> 1, wq = wave & 1, l15 = lane & 15, lg = lane >> 4;
@@ -481,7 +489,7 @@ __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ it
       for (int i = 0; i < PER; ++i) {
         const int c = min((k0 + kt) * 64 + gc[i], ld - 8);  // the last tile may be 32 deep: its second half is not multiplied
         lds_dma16(gp[i] + c, base + buf * (STAGE * 2) + dst[i]);
-        lds_dma16(gq[i] + c, base + buf * (STAGE * 2) + OP * 2 + dst[i]);
+        if (!diag) lds_dma16(gq[i] + c, base + buf * (STAGE * 2) + OP * 2 + dst[i]);
       }
     };
     int fp[WT], fq[WT];
@@ -489,7 +497,7 @@ __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ it
     for (int i = 0; i < WT; ++i) {  // rows 16 apart share their swizzle: 32 slots further is the chunk with bit 2 flipped
       const int rp = (wp * WT + i) * 16 + l15, rq = (wq * WT + i) * 16 + l15;
       fp[i] = rp * 64 + nt_chunk(rp, lg) * 8;
-      fq[i] = OP + rq * 64 + nt_chunk(rq, lg) * 8;
+      fq[i] = (diag ? 0 : OP) + rq * 64 + nt_chunk(rq, lg) * 8;
     }
     const int nk = k1 - k0;
 #pragma unroll
@@ -497,7 +505,8 @@ __global__ __launch_bounds__(256, 2) void k_orth_sym(const Item* __restrict__ it
       if (st < nk) issue(st, st);
     int buf = 0;
     for (int kt = 0; kt < nk; ++kt) {
-      wait_stage<2 * PER, NB>(min(nk - 1 - kt, NB - 2));
+      if (diag) wait_stage<PER, NB>(min(nk - 1 - kt, NB - 2));
+      else wait_stage<2 * PER, NB>(min(nk - 1 - kt, NB - 2));
       __syncthreads();
       if (kt + NB - 1 < nk) issue(kt + NB - 1, buf == 0 ? NB - 1 : buf - 1);
       const f16* s = sm + buf * STAGE;
@@ -1256,7 +1265,8 @@ void plan_grids(const Item& i, int wt_gram, int wt_full, bool mom, int64_t* g) {
 }
 
 // A of long matrices (a contraction of 2048 and more): 128-wide tiles where they are many, the contraction cut into slices of
-// at least 512 until about 512 workgroups share the work.  Measured, slices and 64-wide tiles against the uncut form:
+// at least 512 until about 512 workgroups share the work.  Five steps, uncut / cut: 16 x 8192 302 / 97 us, 400 x 8192
+// 429 / 190 us, 1024 x 4096 349 / 274 us, 2048 x 8192 (128-wide tiles) 961 / 875 us
 void plan_slices(Plan& P) {  // grid[P_GRAM] holds 128-wide tiles
   P.wt_gram = 2;
   P.slices = 1;
@@ -1354,15 +1364,20 @@ void apply(const Plan& P, const Ptrs& p, int cur, int otype, const Momentum& mo,
   hipLaunchKernelGGL((k_orth_apply<MODE, WT, NB>), dim3((unsigned)P.grid[G]), dim3(256), 0, s, p.items, p.end(G), p.count, cur,
                      otype, p.ws, mo);
 }
+// up to two workgroups a CU: three stages of each in flight in place of more workgroups.  Five steps of 1024 x 1024 (136
+// tiles) 185 -> 170 us, of 251 x 1003 (10 tiles) 122 -> 113 us; 12 x 512 x 4096 keeps two stages, which are faster there
+constexpr int64_t FEW_TILES = 512;
 template <int MODE>
 int run_steps(const Plan& P, const Ptrs& p, int steps, int otype, const Momentum& mo, hipStream_t s) {
   const bool only_last = P.grid[P_FULL] == 0;  // small matrices alone: their steps are made
   for (int k = only_last ? steps - 1 : 0, cur = 0; k < steps; ++k, cur ^= 1) {
     if (!only_last) {
-      if (P.slices == 1) sym<GRAM, 2, 2>(P, p, P_GRAM, cur, s);
+      if (P.slices == 1 && P.grid[P_GRAM] <= FEW_TILES) sym<GRAM, 2, 4>(P, p, P_GRAM, cur, s);
+      else if (P.slices == 1) sym<GRAM, 2, 2>(P, p, P_GRAM, cur, s);
       else if (P.wt_gram == 4) { sym<PART, 4, 2>(P, p, P_GRAM, cur, s); sym<JOIN, 4, 2>(P, p, P_GRAM, cur, s); }
       else { sym<PART, 2, 2>(P, p, P_GRAM, cur, s); sym<JOIN, 2, 2>(P, p, P_GRAM, cur, s); }
-      sym<POLY, 2, 2>(P, p, P_POLY, cur, s);
+      if (P.grid[P_POLY] <= FEW_TILES) sym<POLY, 2, 4>(P, p, P_POLY, cur, s);
+      else sym<POLY, 2, 2>(P, p, P_POLY, cur, s);
     }
     if (k + 1 < steps) {
       if (P.wt_full == 4) apply<MID, 4, 2>(P, p, cur, otype, mo, s);
