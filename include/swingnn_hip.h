@@ -460,7 +460,7 @@ int swg_adam_ema_step(const void* p_ptrs, const void* g_ptrs, const int32_t* num
 
 /* ---- layer norm as an operator (no counterpart in the reference beyond nn.LayerNorm) ------------------------ *
  * y = (x - mean) / sqrt(var + eps) * w + b over rows of D elements.  x, y, dy, dx: xtype (SWG_F32 / SWG_BF16 /
- * SWG_F16), unit stride along D, row strides ld* in ELEMENTS (ldx and lddy may be 0: one row for all); no alignment
+ * SWG_F16; outputs may not overlap inputs), unit stride along D, row strides ld* in ELEMENTS (ldx and lddy may be 0: one row for all); no alignment
  * beyond the element's is needed.  w, b [D] or NULL: wtype, SWG_F32 or xtype.  D <= 2^24, rows < 2^31.
  * swg_layer_norm_fwd: mean, rstd [rows] fp32 are written for the backward pass, or both NULL.
  * swg_layer_norm_bwd: dx, dw, db may be NULL; dw, db come in wtype, summed over the rows in fp32 in an order that
@@ -477,7 +477,7 @@ int swg_layer_norm_bwd(int64_t rows, int32_t D, const void* x, int64_t ldx, cons
  * Newton-Schulz: X0 = G / (|G|_F + eps), then `steps` (1 .. 64) times X <- a X + (b A + c A A) X with A = X X' and
  * (a, b, c) = (3.4445, -4.7750, 2.0315).  A zero matrix gives zero; a NaN or infinity in a matrix makes it NaN.
  * swg_orthogonalise: `count` entries (HOST array) of `batch` matrices each, any mix of shapes (rows, cols <= 2^20, 0
- *   allowed); unit stride along a row, row strides ld_* >= cols and matrix strides bs_* in elements.  itype: SWG_F32 /
+ *   allowed); eps > 0 unless no matrix is zero; unit stride along a row, row strides ld_* >= cols and matrix strides bs_* in elements.  itype: SWG_F32 /
  *   SWG_BF16 / SWG_F16; otype: SWG_BF16 / SWG_F16 (the products carry 11 bits, so there is no fp32 output).  Outputs
  *   may not overlap inputs.  ws: swg_orthogonalise_workspace_bytes() of the same entries (0 = unsupported).
  * swg_muon_table: writes the DEVICE table of an optimizer's matrices once (swg_muon_table_bytes(count)); its entries
@@ -489,7 +489,7 @@ int swg_layer_norm_bwd(int64_t rows, int32_t D, const void* x, int64_t ldx, cons
  *   m [total], ema [n_ema, total] at flat_off.  The matrix must not appear twice.
  *   sqnorm (or NULL: no clip) is written first: the sum of squares of every gradient of the entries and of the other
  *   parameters, whose chunks numel / chunk_tensor / chunk_off (n_chunks, may be 0) name as for swg_grad_sqnorm; fp64
- *   partial sums joined in a fixed order (equal inputs, equal bits).  ws: 256-byte aligned. */
+ *   partial sums joined in a fixed order (equal inputs, equal bits).  ws: 256-byte aligned, table: 16-byte. */
 typedef struct swg_orth_item {
   const void* g;
   void* out;

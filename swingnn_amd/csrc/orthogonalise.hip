@@ -1355,8 +1355,9 @@ Ptrs ptrs_of(int count, const Plan& P, const void* table, void* ws) {
 
 template <int KIND, int WT, int NB>
 void sym(const Plan& P, const Ptrs& p, int g, int cur, hipStream_t s) {
-  hipLaunchKernelGGL((k_orth_sym<KIND, WT, NB>), dim3((unsigned)(P.grid[g] * (KIND == PART ? P.slices : KIND == JOIN ? WT : 1))), dim3(256), 0, s,
-                     p.items, p.end(g), p.count, cur, P.slices, p.slices, p.ws);
+  const int64_t per_tile = KIND == PART ? P.slices : KIND == JOIN ? WT : 1;
+  hipLaunchKernelGGL((k_orth_sym<KIND, WT, NB>), dim3((unsigned)(P.grid[g] * per_tile)), dim3(256), 0, s, p.items, p.end(g),
+                     p.count, cur, P.slices, p.slices, p.ws);
 }
 template <int MODE, int WT, int NB>
 void apply(const Plan& P, const Ptrs& p, int cur, int otype, const Momentum& mo, hipStream_t s) {
@@ -1479,7 +1480,7 @@ int swg_muon_table(int32_t count, const swg_muon_item* items, void* table, size_
   if (!muon_plan(count, items, P)) return SWG_E_SHAPE;
   for (int i = 0; i < count; ++i)
     if (items[i].rows < 1 || items[i].cols < 1 || items[i].flat_off < 0 || items[i].index < 0) return SWG_E_SHAPE;
-  if (table_size < table_bytes(count)) return SWG_E_WORKSPACE;
+  if (table_size < table_bytes(count) || ((size_t)table & 15)) return SWG_E_WORKSPACE;
   return write_table(count, P, true, [&](int i, Plan& run, Item& I) {
     plan_item(run, items[i].rows, items[i].cols, 1, true, &I);
     I.flat_off = items[i].flat_off; I.index = items[i].index; I.scale = items[i].scale;
@@ -1497,7 +1498,7 @@ int swg_muon_ema_step(int32_t count, const swg_muon_item* items, const void* tab
   if (sqnorm && n_chunks > 0 && (!numel || !chunk_tensor || !chunk_off)) return SWG_E_NULL;
   Plan P;
   if (!muon_plan(count, items, P)) return SWG_E_SHAPE;
-  if (ws_bytes < ws_bytes_of(P)) return SWG_E_WORKSPACE;
+  if (ws_bytes < ws_bytes_of(P) || ((size_t)ws & 255) || ((size_t)table & 15)) return SWG_E_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
   const Ptrs p = ptrs_of(count, P, table, ws);
   Momentum mo = {};

@@ -16,8 +16,8 @@ _TYPE = {torch.float32: L.SWG_F32, torch.bfloat16: L.SWG_BF16, torch.float16: L.
 def orthogonalise(g, steps=5, eps=1e-7, out_dtype=torch.bfloat16):
     """Orthogonalised matrices of ``g``: a tensor [rows, cols] or [batch, rows, cols], or a list of such tensors of any
     shapes (one type, one device), which go through the same launches.  float32, bfloat16 or float16 in; bfloat16 or
-    float16 out (the products carry 11 bits).  A zero matrix gives zero.  Not differentiable: the result carries no
-    gradient.  The work is queued on the current stream and may be recorded into a graph."""
+    float16 out (the products carry 11 bits).  A zero matrix gives zero.  Not differentiable: a matrix that asks for a
+    gradient is refused in grad mode.  The work is queued on the current stream and may be recorded into a graph."""
     single = isinstance(g, torch.Tensor)
     mats = [g] if single else list(g)
     if not 1 <= int(steps) <= 64:
@@ -33,6 +33,8 @@ def orthogonalise(g, steps=5, eps=1e-7, out_dtype=torch.bfloat16):
             raise NotImplementedError(f"orthogonalise: float32, bfloat16 or float16, got {t.dtype}")
         if t.dtype is not mats[0].dtype or t.device != mats[0].device:
             raise ValueError("orthogonalise: matrices of one type on one device")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("orthogonalise has no gradient: call it under torch.no_grad() or on a detached matrix")
         if t.device.type != "cuda":
             raise RuntimeError("swingnn_amd runs on an MI355X only; there is no CPU fallback")
     if not mats:

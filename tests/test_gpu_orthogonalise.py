@@ -104,7 +104,8 @@ def test_large_tiles():
     _check(h, S.orthogonalise(h))
 
 
-@pytest.mark.parametrize("shape", [(16, 4096), (130, 2500), (2048, 257), (65, 8192), (700, 2049), (2, 300, 2048), (1800, 2300)])
+@pytest.mark.parametrize("shape", [(16, 4096), (130, 2500), (2048, 257), (65, 8192), (700, 2049), (2, 300, 2048), (1800, 4100),
+                                   (4097, 1700)])
 def test_long_contractions(shape):
     """A cut along the contraction: slices of uneven length, 64- and 128-wide tiles, batches, both orientations."""
     import swingnn_amd as S

@@ -77,6 +77,8 @@ def test_orthogonalise_refusals(S):
         S.orthogonalise(g, eps=-1.0)
     with pytest.raises((ValueError, RuntimeError)):
         S.orthogonalise([g, g.half()])
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        S.orthogonalise(g.clone().requires_grad_(True))
     assert S.orthogonalise([]) == []
 
 
@@ -140,7 +142,7 @@ def test_muon_refusals(S):
     ok = [1, items, p, p, p, p, p, 64, 0, None, p, p, p, 1, p, 0.0, 1e-3, 0.9, 1, 0.0, 5, 1e-7, p, 1 << 20, None]
     for at, bad, code in ((0, 0, -1), (7, 0, -1), (8, 9, -1), (13, -1, -1), (20, 0, -1), (20, 65, -1), (21, -1.0, -1), (1, None, -4), (2, None, -4),
                           (3, None, -4), (4, None, -4), (5, None, -4), (10, None, -4), (11, None, -4), (12, None, -4), (22, None, -4),
-                          (23, 64, -3), (8, 1, -4)):
+                          (23, 64, -3), (8, 1, -4), (22, p + 16, -3), (2, p + 8, -3)):
         args = list(ok)
         args[at] = bad
         assert st(*args) == code, at
