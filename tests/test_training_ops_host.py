@@ -3,6 +3,13 @@ import pytest
 import torch
 
 
+@pytest.fixture(autouse=True)
+def _grad_mode():
+    """Other modules of the suite switch gradients off for the process."""
+    with torch.enable_grad():
+        yield
+
+
 @pytest.fixture(scope="module")
 def S():
     import swingnn_amd
