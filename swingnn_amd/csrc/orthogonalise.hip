@@ -429,6 +429,9 @@ __device__ __forceinline__ int nt_chunk(int row, int ch) { return ch ^ (row & 7)
 // A or B: T x T tile of a symmetric product P P' of one operand with contiguous contraction, T = 32 WT, 4 waves of
 // 16 WT x 16 WT.  64-deep tiles of both row panels (whole 128-byte lines) go to LDS by LDS-DMA, NB stages.  What bounds it is
 // the stream from L2 into LDS, about 14 TB/s: 32 flop per byte at T = 64 (460 TFLOP/s measured), 64 at T = 128.
+// Whole calls of five steps, both sides in turn: tiles staged through registers two ahead instead of by LDS-DMA 222 against
+// 169 us (1024^2), 924 against 846 us (2048 x 8192); both halves' fragments read before the products 175 against 170 and
+// 860 against 852 us; eight stages where tiles are few 175 against 170 us (1024^2).
 // PART / JOIN: few tiles of a long contraction.  PART: workgroup (slice, tile) writes its accumulators as they lie; JOIN adds
 // a tile's slices in order and goes on as GRAM does.
 enum { GRAM = 0, POLY, PART, JOIN };
