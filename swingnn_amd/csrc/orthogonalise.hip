@@ -167,6 +167,13 @@ __device__ __forceinline__ void swap_rows(f16x4& a, f16x4& b) {
 }
 __device__ __forceinline__ int swapped_col(int lg) { return 8 * (lg >> 1) + 16 * (lg & 1); }
 
+// Where m and g nearly cancel, u is the rounding of its own fp32 sums and |u|^2 from the three sums the rounding of
+// theirs; their quotient has no bound (1.5e6 in an emulation of 300 x 400), and above 1.2024 the quintic diverges.  |u|^2
+// is therefore taken as at least 2^-34 of R^2 = (ca |m|)^2 + (cb |g|)^2.  u carries at most six roundings of either term,
+// 6 2^-24 sqrt(2) R in all; fp64 sums of k terms in a chain move |u| by sqrt(k) 2^-26.5 sqrt(2) R: together below 0.2 of
+// 2^-17 R for k < 4600 (up to 10^9 elements), so |X0| < 1.2.  Updates above 2^-17 R are what they were.
+constexpr double CANCEL = 1.0 / (1ull << 34);
+
 __device__ __forceinline__ double block_sum(double s, double* red) {  // 256 threads; all get the sum
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -377,8 +384,9 @@ __global__ __launch_bounds__(256) void k_orth_init(const Item* __restrict__ item
     mx = block_sum(mx, red);
     // u = ca m + cb g of the old m
     const double mu = mo.mu, ca = mo.nesterov ? mu * mu : mu, cb = (mo.nesterov ? (1.0 - mu) * (1.0 + mu) : 1.0 - mu) * clip;
+    const double least = (ca * ca * mx + cb * cb * s) * CANCEL;
     s = ca * ca * mx + 2.0 * ca * cb * gx + cb * cb * s;
-    s = s < 0.0 ? 0.0 : s;  // a NaN stays
+    s = s < least ? least : s;  // a NaN stays
   }
   const double inv = (double)SX / (sqrt(s) + eps);
   if (tall) {
