@@ -7,9 +7,8 @@
 //
 // Both passes are bound by HBM: x is read once and y written once; backward reads x and dy and writes dx.  A row is held
 // in the registers of LANES lanes (8 .. 64: several rows per wavefront; 256 .. 1024: one row per workgroup) as V chunks
-// of N elements (16 bytes), so mean and variance are two sums over registers (the variance of the centred values: no
-// cancellation).  Both are divided by D, not multiplied by 1 / D, whose rounding would leave a residue of equal values
-// that r = 1 / sqrt(eps) makes visible.
+// of N elements (16 bytes), so mean and variance are two sums over registers: the mean's in 64 bits, the variance's of the
+// centred values (no cancellation).  The backward pass reads the mean rounded to 32 bits.
 // Loads carry the alignment of the ELEMENT only: gfx950 serves 16-byte loads at any address, so odd widths and row
 // strides take the same path.  The last chunk of a width that N does not divide is moved back to end with the row: it
 // overlaps its neighbour, whose columns it leaves out of the sums and stores a second time with the same values.
@@ -19,6 +18,7 @@
 // Measured (a large copy reaches 5.0 TB/s): forward 516096 x 96 fp32 78 us (5.1 TB/s), backward 184320 x 192 fp32 84 us
 // (5.1 TB/s of x, dy, dx), 8192 x 4096 bf16 forward 26 us (5.1 TB/s), backward 45 us (4.5 TB/s and 34 MB of partial sums).
 #include "common.h"
+#include <type_traits>
 
 namespace {
 
@@ -64,25 +64,89 @@ struct Cols {
 
 __device__ __forceinline__ int cdiv_dev(int a, int b) { return (a + b - 1) / b; }
 
+// group_sum() of common.h in 64 bits: both halves of the number move by the same register exchanges
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+  const uint2 u = __builtin_bit_cast(uint2, v);
+  const uint2 o = make_uint2(__builtin_amdgcn_update_dpp(0u, u.x, CTRL, 0xf, 0xf, false),
+                             __builtin_amdgcn_update_dpp(0u, u.y, CTRL, 0xf, 0xf, false));
+  return v + __builtin_bit_cast(double, o);
+}
+template <int LANES>
+__device__ __forceinline__ double group_sum(double v) {
+  if constexpr (LANES >= 16) {
+    if constexpr (LANES == 64) {
+      const uint2 u = __builtin_bit_cast(uint2, v);
+      const auto x = __builtin_amdgcn_permlane32_swap(u.x, u.x, false, false), y = __builtin_amdgcn_permlane32_swap(u.y, u.y, false, false);
+      v = __builtin_bit_cast(double, make_uint2(x[0], y[0])) + __builtin_bit_cast(double, make_uint2(x[1], y[1]));
+    }
+    if constexpr (LANES >= 32) {
+      const uint2 u = __builtin_bit_cast(uint2, v);
+      const auto x = __builtin_amdgcn_permlane16_swap(u.x, u.x, false, false), y = __builtin_amdgcn_permlane16_swap(u.y, u.y, false, false);
+      v = __builtin_bit_cast(double, make_uint2(x[0], y[0])) + __builtin_bit_cast(double, make_uint2(x[1], y[1]));
+    }
+    v = dpp_add<0x128>(v);  // row_ror:8, 4, 2, 1
+    v = dpp_add<0x124>(v);
+    v = dpp_add<0x122>(v);
+    v = dpp_add<0x121>(v);
+  } else {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  }
+  return v;
+}
+
 // Sum over the LANES lanes of a row.  LANES > 64: the whole workgroup; `red` alternates between two slots per call so
 // that one barrier a call is enough.
-template <int LANES>
-__device__ __forceinline__ float row_sum(float v, float* red, int& slot) {
+template <int LANES, class A>
+__device__ __forceinline__ A row_sum(A v, A* red, int& slot) {
   if constexpr (LANES <= 64) {
     return group_sum<LANES>(v);
   } else {
     constexpr int W = LANES / 64;
     v = group_sum<64>(v);
-    float* r = red + slot * W;
+    A* r = red + slot * W;
     slot ^= 1;
     if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
     __syncthreads();
-    float s = 0.f;
+    if constexpr (sizeof(A) == 8) {  // a 64-bit add takes longer: log2(W) of them in a chain, not W
+      A t[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) t[i] = r[i];
+#pragma unroll
+      for (int n = W / 2; n > 0; n /= 2)
+#pragma unroll
+        for (int i = 0; i < n; ++i) t[i] += t[i + n];
+      return t[0];
+    }
+    A s = 0;
 #pragma unroll
     for (int i = 0; i < W; ++i) s += r[i];
     return s;
   }
 }
+
+// The mean of a row from its sum in 64 bits, as a pair hi + lo: x - hi is exact for x near the mean, so x - hi - lo is as
+// exact for a mean of 30000 as for one of 0.  A float32 sum leaves a few steps of the mean in every element, which
+// r <= 1 / sqrt(eps) = 316 multiplies (rows of values around 30000.7, a few steps apart: y off by up to 3.3).  Sums of equal
+// values are exact here (24 + 24 bits), and so is s - D hi.  `inv` is 1 / D.  Float32 / 64-bit sums: 516096 x 96 fp32
+// 74.0 / 75.1 us, 184320 x 192 47.0 / 47.9 us, 8192 x 4096 bf16 24.1 / 24.9 us, 4096 x 16384 fp32 111.9 / 117.4 us.
+// A chunk of a half type (11 bits at most) is summed in float32 first, which is exact for values within a factor of two.
+template <class T, int N>
+__device__ __forceinline__ double chunk_sum(const float* v, int lo) {  // of the elements from `lo` on
+  typedef std::conditional_t<sizeof(T) == 2, float, double> A;
+  A s = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) s += (A)(e >= lo ? v[e] : 0.f);
+  return (double)s;
+}
+struct Mean {
+  float hi, lo;
+  __device__ __forceinline__ Mean(double s, int D, double inv) {
+    hi = (float)(s * inv);
+    lo = (float)((s - (double)D * (double)hi) * inv);
+  }
+};
 
 template <int LANES>
 constexpr int block_of() { return LANES <= 64 ? 256 : LANES; }
@@ -95,8 +159,10 @@ __global__ __launch_bounds__(block_of<LANES>()) void k_ln_fwd(const T* __restric
                                                               float* __restrict__ rstd_out) {
   constexpr int BLK = block_of<LANES>(), RPB = BLK / LANES;
   __shared__ float red[2 * (LANES > 64 ? LANES / 64 : 1)];
+  __shared__ double red_mean[2 * (LANES > 64 ? LANES / 64 : 1)];
   const int gl = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   const bool ragged = D != N * LANES * V;
+  const double inv = 1.0 / (double)D;
   int slot = 0;
   // the bound is the same for all lanes of a workgroup, so every barrier inside is reached by all of them
   for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < rows; row0 += (int64_t)gridDim.x * RPB) {
@@ -104,26 +170,20 @@ __global__ __launch_bounds__(block_of<LANES>()) void k_ln_fwd(const T* __restric
     const bool live = row0 + grp < rows;
     const T* xr = x + row * ldx;
     float v[V][N];
-    float s = 0.f;
+    double s = 0.0;
 #pragma unroll
     for (int i = 0; i < V; ++i) load_vec<T, N>(xr + Cols<N>(gl + LANES * i, D).col, v[i]);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (ragged) {
-        const int lo = Cols<N>(gl + LANES * i, D).lo;
-#pragma unroll
-        for (int e = 0; e < N; ++e) s += e >= lo ? v[i][e] : 0.f;
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) s += v[i][e];
-      }
+      if (ragged) s += chunk_sum<T, N>(v[i], Cols<N>(gl + LANES * i, D).lo);
+      else s += chunk_sum<T, N>(v[i], 0);
     }
-    const float mean = row_sum<LANES>(s, red, slot) / (float)D;
+    const Mean mean(row_sum<LANES>(s, red_mean, slot), D, inv);
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[i][e] -= mean;
+      for (int e = 0; e < N; ++e) v[i][e] = (v[i][e] - mean.hi) - mean.lo;
       if (ragged) {
         const int lo = Cols<N>(gl + LANES * i, D).lo;
 #pragma unroll
@@ -152,7 +212,7 @@ __global__ __launch_bounds__(block_of<LANES>()) void k_ln_fwd(const T* __restric
         if (c.lo < N) store_vec<T, N>(yr + c.col, v[i]);
       }
       if (mean_out && gl == 0) {
-        mean_out[row] = mean;
+        mean_out[row] = mean.hi;
         rstd_out[row] = rstd;
       }
     }
@@ -166,23 +226,28 @@ __global__ __launch_bounds__(1024) void k_ln_fwd_wide(const T* __restrict__ x, i
                                                       T* __restrict__ y, int64_t ldy, float* __restrict__ mean_out,
                                                       float* __restrict__ rstd_out) {
   __shared__ float red[32];
+  __shared__ double red_mean[32];
   const int nch = cdiv_dev(D, N);
+  const double inv = 1.0 / (double)D;
   int slot = 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* xr = x + row * ldx;
-    float s = 0.f, q = 0.f, v[N];
+    double s = 0.0;
+    float q = 0.f, v[N];
     for (int c = threadIdx.x; c < nch; c += 1024) {
       const Cols<N> cc(c, D);
       load_vec<T, N>(xr + cc.col, v);
-#pragma unroll
-      for (int e = 0; e < N; ++e) s += e >= cc.lo ? v[e] : 0.f;
+      s += chunk_sum<T, N>(v, cc.lo);
     }
-    const float mean = row_sum<1024>(s, red, slot) / (float)D;
+    const Mean mean(row_sum<1024>(s, red_mean, slot), D, inv);
     for (int c = threadIdx.x; c < nch; c += 1024) {
       const Cols<N> cc(c, D);
       load_vec<T, N>(xr + cc.col, v);
 #pragma unroll
-      for (int e = 0; e < N; ++e) q += e >= cc.lo ? (v[e] - mean) * (v[e] - mean) : 0.f;
+      for (int e = 0; e < N; ++e) {
+        const float c = (v[e] - mean.hi) - mean.lo;
+        q += e >= cc.lo ? c * c : 0.f;
+      }
     }
     const float rstd = 1.0f / sqrtf(row_sum<1024>(q, red, slot) / (float)D + eps);
     for (int c = threadIdx.x; c < nch; c += 1024) {
@@ -193,14 +258,14 @@ __global__ __launch_bounds__(1024) void k_ln_fwd_wide(const T* __restrict__ x, i
       if (b) load_vec<TW, N>(b + cc.col, bb);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        v[e] = (v[e] - mean) * rstd;
+        v[e] = ((v[e] - mean.hi) - mean.lo) * rstd;
         if (w) v[e] *= ww[e];
         if (b) v[e] += bb[e];
       }
       store_vec<T, N>(y + row * ldy + cc.col, v);
     }
     if (mean_out && threadIdx.x == 0) {
-      mean_out[row] = mean;
+      mean_out[row] = mean.hi;
       rstd_out[row] = rstd;
     }
   }
