@@ -9,6 +9,8 @@ import ctypes as C
 import os
 
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib as L
 
@@ -30,6 +32,18 @@ def _ptr(t):
 
 def stream_ptr():
     return torch.cuda.current_stream().cuda_stream
+
+
+def refuse_transforms(what, tensors):
+    """Operators queue their work through raw pointers: a forward-mode tangent would be dropped and a trace would record
+    the allocations alone, so both are refused.  (func.grad, func.jvp and vmap raise by themselves; autograd.Function
+    carries reverse mode.)"""
+    if torch.jit.is_tracing() or get_proxy_mode() is not None:
+        raise NotImplementedError(f"{what} cannot be traced (torch.jit.trace, make_fx): its kernels are not torch operations")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative: use reverse mode, or a tensor without a tangent")
 
 
 def call_on(device, fn, what, *args):

@@ -14,7 +14,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from .engine import call_on
+from .engine import call_on, refuse_transforms
 
 _TYPE = {torch.float32: L.SWG_F32, torch.bfloat16: L.SWG_BF16, torch.float16: L.SWG_F16}
 
@@ -97,7 +97,9 @@ class _LayerNormFn(torch.autograd.Function):
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """Layer norm of ``x`` over its last axis; differentiable once."""
+    """Layer norm of ``x`` over its last axis; differentiable once, in reverse mode (a forward-mode tangent, a trace and a
+    second derivative are refused)."""
+    refuse_transforms("layer_norm", (x, weight, bias))
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"layer_norm: a last axis to normalise is needed, got shape {tuple(x.shape)}")
     if x.dtype not in _TYPE:

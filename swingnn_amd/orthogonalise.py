@@ -8,7 +8,7 @@ singular vectors: about U V' of G = U S V'.
 import torch
 
 from . import _lib as L
-from .engine import call_on
+from .engine import call_on, refuse_transforms
 
 _TYPE = {torch.float32: L.SWG_F32, torch.bfloat16: L.SWG_BF16, torch.float16: L.SWG_F16}
 
@@ -17,9 +17,10 @@ def orthogonalise(g, steps=5, eps=1e-7, out_dtype=torch.bfloat16):
     """Orthogonalised matrices of ``g``: a tensor [rows, cols] or [batch, rows, cols], or a list of such tensors of any
     shapes (one type, one device), which go through the same launches.  float32, bfloat16 or float16 in; bfloat16 or
     float16 out (the products carry 11 bits).  A zero matrix gives zero.  Not differentiable: a matrix that asks for a
-    gradient is refused in grad mode.  The work is queued on the current stream and may be recorded into a graph."""
+    gradient in grad mode, one with a forward-mode tangent and a trace are refused.  The work is queued on the current stream and may be recorded into a graph."""
     single = isinstance(g, torch.Tensor)
     mats = [g] if single else list(g)
+    refuse_transforms("orthogonalise", mats)
     if not 1 <= int(steps) <= 64:
         raise ValueError("orthogonalise: steps between 1 and 64")
     if not eps >= 0.0:
