@@ -72,7 +72,8 @@ __global__ __launch_bounds__(256) void k_adam_ema(AdamArgs a) {
   const int64_t fo = a.flat_off[t] + off;
   float clip = 1.f;
   if (a.sqnorm) {  // torch.nn.utils.clip_grad_norm_: coef = max_norm / (norm + 1e-6), clamped to 1
-    clip = fminf(a.max_norm / (sqrtf(*a.sqnorm) + 1e-6f), 1.0f);
+    const float c = a.max_norm / (sqrtf(*a.sqnorm) + 1e-6f);
+    clip = c > 1.f ? 1.f : c;  // a NaN norm stays NaN and reaches every gradient, as it does there; fminf would make it 1
   }
   const float step = a.lr / a.bc1;
   auto update = [&](float& pv, float gv, float& mv, float& vv) {
