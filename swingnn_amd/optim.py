@@ -145,24 +145,27 @@ class FusedAdamEMA(torch.optim.Optimizer):
         return self._sqnorm.sqrt().squeeze(0)
 
     def _point(self):
-        """Device tables of the gradients' and parameters' present addresses."""
-        grads = []
-        for p in self.params:
-            g = p.grad
+        """Device tables of the gradients' and parameters' present addresses.  The kernels go by the sizes and the layout
+        of the constructor, so those are checked on every step: ``p.data = p.data.t()`` or ``p.data[:k]`` keeps the address."""
+        T = torch.Tensor
+        params, grads = self.params, [p.grad for p in self.params]
+        for k, g in enumerate(grads):
             if g is None:
                 raise RuntimeError(f"{type(self).__name__}.step: every parameter needs a gradient (the denoiser uses all of them)")
-            if g.dtype != torch.float32 or not g.is_contiguous():
-                g = p.grad = g.to(torch.float32).contiguous()
-            grads.append(g)
-        key = tuple(g.data_ptr() for g in grads)
+            if g.dtype is not torch.float32 or not g.is_contiguous():
+                grads[k] = params[k].grad = g.to(torch.float32).contiguous()
+        if (list(map(T.size, params)) != self._shapes or list(map(T.size, grads)) != self._shapes
+                or not all(map(T.is_contiguous, params))):
+            raise NotImplementedError(f"{type(self).__name__}: parameters and gradients keep their shapes, and parameters stay contiguous")
+        key = tuple(map(T.data_ptr, grads))
         if key != self._g_key:  # zero_grad(set_to_none=True) gives new gradient tensors every step
             self._g_ptrs.copy_(torch.tensor(key, dtype=torch.int64), non_blocking=False)
             self._g_key = key
-        pkey = tuple(p.data_ptr() for p in self.params)
+        pkey = tuple(map(T.data_ptr, params))
         if pkey != self._p_key:  # parameter storage moved (model.to(), p.data = ..., load_state_dict(assign=True))
-            for p, shape in zip(self.params, self._shapes):
-                if p.dtype != torch.float32 or not p.is_contiguous() or p.device != self.m.device or p.shape != shape:
-                    raise NotImplementedError(f"{type(self).__name__}: parameters stay contiguous fp32 of their shape and device")
+            for p in params:
+                if p.dtype != torch.float32 or p.device != self.m.device:
+                    raise NotImplementedError(f"{type(self).__name__}: parameters stay fp32 on their device")
             self._p_ptrs.copy_(torch.tensor(pkey, dtype=torch.int64), non_blocking=False)
             self._p_key = pkey
             self._views = None
