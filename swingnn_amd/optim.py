@@ -129,6 +129,9 @@ class FusedAdamEMA(torch.optim.Optimizer):
         fused = state_dict.pop("fused", None)
         if fused is None:
             raise KeyError(f"{type(self).__name__}.load_state_dict: no 'fused' entry (not a {type(self).__name__} checkpoint)")
+        # both kinds save a "fused" entry, and one without other parameters has one group like Adam's
+        if fused.get("n_matrices") != getattr(self, "n_matrices", None):
+            raise ValueError(f"{type(self).__name__}.load_state_dict: another split into matrices and others than the checkpoint's")
         if list(fused["numel"]) != [p.numel() for p in self.params]:
             raise ValueError(f"{type(self).__name__}.load_state_dict: parameter list differs from the checkpoint's")
         if [float(b) for b in fused["ema_betas"]] != list(self.ema_betas):
@@ -275,12 +278,6 @@ class FusedMuonEMA(FusedAdamEMA):
         sd = super().state_dict()
         sd["fused"]["n_matrices"] = self.n_matrices
         return sd
-
-    def load_state_dict(self, state_dict):
-        fused = state_dict.get("fused")
-        if fused is not None and fused.get("n_matrices") != self.n_matrices:
-            raise ValueError("FusedMuonEMA.load_state_dict: another split into matrices and others than the checkpoint's")
-        super().load_state_dict(state_dict)
 
     @torch.no_grad()
     def step(self, closure=None):
