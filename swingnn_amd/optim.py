@@ -120,7 +120,7 @@ class FusedAdamEMA(torch.optim.Optimizer):
         sd["fused"] = {
             "m": self.m.detach().clone(), "v": self.v.detach().clone(), "ema": self.ema.detach().clone(),
             "step_count": self.step_count, "ema_updates": self.ema_updates, "ema_betas": list(self.ema_betas),
-            "numel": [p.numel() for p in self.params],
+            "numel": [p.numel() for p in self.params], "shapes": [list(s) for s in self._shapes],
         }
         return sd
 
@@ -134,6 +134,9 @@ class FusedAdamEMA(torch.optim.Optimizer):
             raise ValueError(f"{type(self).__name__}.load_state_dict: another split into matrices and others than the checkpoint's")
         if list(fused["numel"]) != [p.numel() for p in self.params]:
             raise ValueError(f"{type(self).__name__}.load_state_dict: parameter list differs from the checkpoint's")
+        shapes = fused.get("shapes")  # older checkpoints hold the sizes alone
+        if shapes is not None and [tuple(s) for s in shapes] != [tuple(s) for s in self._shapes]:
+            raise ValueError(f"{type(self).__name__}.load_state_dict: parameter shapes differ from the checkpoint's")
         if [float(b) for b in fused["ema_betas"]] != list(self.ema_betas):
             raise ValueError(f"{type(self).__name__}.load_state_dict: EMA betas differ from the checkpoint's")
         super().load_state_dict(state_dict)
