@@ -126,7 +126,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 
 class LayerNorm(nn.LayerNorm):
-    """``nn.LayerNorm`` over one axis whose forward is ``layer_norm``."""
+    """``nn.LayerNorm`` over one axis whose forward is ``layer_norm``.  Under autocast it does what ``nn.LayerNorm`` does
+    there: half types are normalised and returned in float32 (``layer_norm`` itself takes what it is given)."""
 
     def __init__(self, *args, **kwargs):
         super().__init__(*args, **kwargs)
@@ -136,4 +137,8 @@ class LayerNorm(nn.LayerNorm):
     def forward(self, x):
         if x.shape[-1:] != self.normalized_shape:
             raise ValueError(f"LayerNorm: last axis {tuple(x.shape)[-1:]}, normalised shape {tuple(self.normalized_shape)}")
-        return layer_norm(x, self.weight, self.bias, self.eps)
+        weight, bias = self.weight, self.bias
+        if torch.is_autocast_enabled("cuda"):
+            x, weight, bias = (t.float() if t is not None and t.dtype in (torch.bfloat16, torch.float16) else t
+                               for t in (x, weight, bias))
+        return layer_norm(x, weight, bias, self.eps)
