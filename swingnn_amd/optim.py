@@ -208,9 +208,11 @@ class FusedAdamEMA(torch.optim.Optimizer):
     def _bump_versions(self):
         """Parameters were updated through raw pointers; bump their version counters so derived weight caches
         (engine.NetCache) rebuild: one foreach call on zero-size views (no element is touched, the counters move).  The
-        views are kept until a parameter's storage moves: making 392 of them took 560 us of a step, using them 37 us."""
+        views are kept until a parameter's storage moves: making 392 of them took 560 us of a step, using them 37 us.  They
+        are views of detached tensors, which share the counter but do not hold the parameter (torch.utils.swap_tensors,
+        and with it module.to() where params are swapped, refuses one that something else holds)."""
         if self._views is None:
-            self._views = [p.view(-1)[:0] for p in self.params]
+            self._views = [p.detach().view(-1)[:0] for p in self.params]
         torch._foreach_add_(self._views, 0.0)
 
 
