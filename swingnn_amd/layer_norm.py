@@ -21,6 +21,8 @@ _TYPE = {torch.float32: L.SWG_F32, torch.bfloat16: L.SWG_BF16, torch.float16: L.
 
 def _rows(t, D):
     """t as [rows, D] with unit stride along D, without a copy where its strides allow it."""
+    if D == 1:
+        t = t.resolve_neg()  # the sign flag of z.conj().imag: for wider rows its stride of two has a copy made, which resolves it
     if t.dim() != 2:
         try:
             t = t.view(-1, D)
@@ -117,6 +119,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         raise NotImplementedError("layer_norm: weight and bias of one type")
     if x.device.type != "cuda":
         raise RuntimeError("swingnn_amd runs on an MI355X only; there is no CPU fallback")
+    if x.shape[-1] == 1:
+        weight, bias = (t if t is None else t.resolve_neg() for t in (weight, bias))
     weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
     bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)

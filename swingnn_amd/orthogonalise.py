@@ -44,7 +44,7 @@ def orthogonalise(g, steps=5, eps=1e-7, out_dtype=torch.bfloat16):
     outs, items, keep = [], (L.SwgOrthItem * len(mats))(), []
     for t, it in zip(mats, items):
         rows, cols = t.shape[-2:]
-        t = t.detach()
+        t = t.detach().resolve_neg()  # z.conj().imag holds its sign as a flag, which a column keeps through the strides below
         # a row of one element has no stride of its own
         if t.numel() and ((cols > 1 and t.stride(-1) != 1) or (rows > 1 and t.stride(-2) < cols)):
             t = t.contiguous()
