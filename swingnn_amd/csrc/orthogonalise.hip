@@ -1313,8 +1313,8 @@ bool make_plan(int32_t count, bool mom, F shape, Plan& P) {  // shape(i, rows, c
       plan_slices(P);
     }
   }
-  for (int k = 0; k < PREFIXES; ++k)
-    if (P.grid[k] > 0x7fffffff) return false;
+  for (int k = 0; k < PREFIXES; ++k)  // a launch holds fewer than 2^32 threads (the norm pass takes OTHER_BLOCKS more)
+    if ((P.grid[k] + OTHER_BLOCKS) * (k == P_SMALL ? 512 : 256) > 0xffffffffll) return false;
   return true;
 }
 
