@@ -97,6 +97,14 @@ __device__ __forceinline__ float group_sum(float v) {
   }
 }
 
+// bijective XCD remap (8 XCDs, round-robin dispatch): logical tile id from hardware block id
+__device__ __forceinline__ int xcd_remap(int bid, int nwg) {
+  const int q = nwg >> 3, r = nwg & 7;
+  const int xcd = bid & 7, slot = bid >> 3;
+  const int start = (xcd < r) ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q;
+  return start + slot;
+}
+
 // Reductions over the four 16-lane rows of a wavefront (lanes l, l^16, l^32, l^48) with the gfx950 row-swap
 // instructions: v_permlane{16,32}_swap exchange register rows in the VALU, no LDS round trip (ds_bpermute costs an
 // LDS latency per step, which one wave per SIMD cannot hide).  Every lane ends with the full result.

@@ -28,14 +28,6 @@ struct Swz {
   }
 };
 
-// bijective XCD remap (8 XCDs, round-robin dispatch): logical tile id from hardware block id
-__device__ __forceinline__ int xcd_remap(int bid, int nwg) {
-  const int q = nwg >> 3, r = nwg & 7;
-  const int xcd = bid & 7, slot = bid >> 3;
-  const int start = (xcd < r) ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q;
-  return start + slot;
-}
-
 // BMT: token rows per block tile.  128 (4 x 4 MFMA tiles per wave) is the default; 64 (2 x 4 per wave) doubles the
 // workgroup count for shapes that would otherwise put one or two workgroups on a CU: with so few waves the
 // register-staged pipeline exposes a memory latency per k-step (C = 768 fc2 at M = 8064: 378 workgroups, 70 us for

@@ -98,11 +98,6 @@ __device__ __forceinline__ int find_item(const int32_t* __restrict__ ends, int n
 }
 
 __device__ __forceinline__ int cdiv_up(int a, int b) { return (a + b - 1) / b; }
-__device__ __forceinline__ int xcd_remap(int bid, int nwg) {
-  const int q = nwg >> 3, r = nwg & 7;
-  const int xcd = bid & 7, slot = bid >> 3;
-  return ((xcd < r) ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + slot;
-}
 
 struct Bufs {
   char* x;
