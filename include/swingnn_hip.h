@@ -479,14 +479,16 @@ int swg_layer_norm_bwd(int64_t rows, int32_t D, const void* x, int64_t ldx, cons
  * swg_orthogonalise: `count` entries (HOST array) of `batch` matrices each, any mix of shapes (rows, cols <= 2^20, 0
  *   allowed); eps > 0 unless no matrix is zero; unit stride along a row, row strides ld_* >= cols and matrix strides bs_* in elements.  itype: SWG_F32 /
  *   SWG_BF16 / SWG_F16; otype: SWG_BF16 / SWG_F16 (the products carry 11 bits, so there is no fp32 output).  Outputs
- *   may not overlap inputs.  ws: swg_orthogonalise_workspace_bytes() of the same entries (0 = unsupported).
+ *   may not overlap inputs.  ws: swg_orthogonalise_workspace_bytes() of the same entries (0 = unsupported, as where a
+ *   launch would reach 2^32 threads: 8.3 M matrices of the one-workgroup size, 16.7 M tiles of others).
  * swg_muon_table: writes the DEVICE table of an optimizer's matrices once (swg_muon_table_bytes(count)); its entries
  *   name a matrix by its place in the pointer tables, so gradients and parameters may move between steps.
  * swg_muon_ema_step, for every entry (same HOST array as the table's):
- *   g <- g min(1, max_norm / (sqrt(*sqnorm) + 1e-6)) when sqnorm != NULL;  m <- momentum m + (1 - momentum) g;
+ *   g <- g min(1, max_norm / (sqrt(*sqnorm) + 1e-6)) when sqnorm != NULL (NaN stays NaN);  m <- momentum m + (1 - momentum) g;
  *   u = nesterov ? momentum m + (1 - momentum) g : m;  p <- p (1 - lr weight_decay) - lr scale orthogonalise(u);
  *   ema_k <- lerp(ema_k, p, 1 - ema_decay[k]) (ema_decay: HOST array).  p, g: DEVICE pointer tables, contiguous fp32;
- *   m [total], ema [n_ema, total] at flat_off.  The matrix must not appear twice.
+ *   m [total], ema [n_ema, total] at flat_off.  The matrix must not appear twice.  |u| counts as at least 2^-17 of its
+ *   terms' size, so an m and g that cancel to rounding move p by no more than an orthogonal matrix does.
  *   sqnorm (or NULL: no clip) is written first: the sum of squares of every gradient of the entries and of the other
  *   parameters, whose chunks numel / chunk_tensor / chunk_off (n_chunks, may be 0) name as for swg_grad_sqnorm; fp64
  *   partial sums joined in a fixed order (equal inputs, equal bits).  ws: 256-byte aligned, table: 16-byte. */

@@ -15,8 +15,9 @@
 // Backward: lane and chunk fix the columns, so every lane sums dw / db of its columns over the rows of its workgroup in
 // registers; the row groups of a workgroup are joined by shuffles and LDS, the workgroups by k_ln_cols.  The next row's
 // x and dy are loaded before the present row's sums where the registers hold both.
-// Measured (a large copy reaches 5.0 TB/s): forward 516096 x 96 fp32 78 us (5.1 TB/s), backward 184320 x 192 fp32 84 us
-// (5.1 TB/s of x, dy, dx), 8192 x 4096 bf16 forward 26 us (5.1 TB/s), backward 45 us (4.5 TB/s and 34 MB of partial sums).
+// Measured (a large copy reaches 4.9 TB/s; kernel times under rocprofv3): forward 516096 x 96 fp32 76 us (5.2 TB/s; part of
+// x stays in the memory-side cache), backward 184320 x 192 fp32 89 us (4.8 TB/s of x, dy, dx), 8192 x 4096 bf16 forward
+// 26 us (5.1 TB/s), backward 53 us (3.8 TB/s, and 34 MB of partial sums), 4097 x 1001 fp16 forward 7, backward 16 + 4 us.
 #include "common.h"
 #include <type_traits>
 
@@ -538,8 +539,8 @@ int bwd_blocks(int64_t rows, int D, int form) {
   if (form < 0) return (int)(rows < 64 ? rows : 64);  // slabs of k_ln_bwd_cols_wide
   const int rpb = kLanes[form] <= 64 ? 256 / kLanes[form] : 1;
   const int64_t need = (rows + rpb - 1) / rpb;
-  // two workgroups a CU.  Time of k_ln_bwd_rows (184320 x 192 fp32 / 8192 x 4096 bf16) with the next row's loads in
-  // flight: 256 workgroups 91 / 51 us, 512: 84 / 45 us, 1024: 101 / 56 us; without them 1024 were best: 91 / 59 us
+  // two workgroups a CU.  Time of k_ln_bwd_rows in a sweep of its own (184320 x 192 fp32 / 8192 x 4096 bf16) with the next
+  // row's loads in flight: 256 workgroups 91 / 51 us, 512: 84 / 45 us, 1024: 101 / 56 us; without them 1024 were best: 91 / 59 us
   return (int)(need < 512 ? need : 512);
 }
 

@@ -2,28 +2,35 @@
 //
 //   X0 = G / (|G|_F + eps);   X <- a X + (b A + c A A) X  with  A = X X',  `steps` times
 //
-// with (a, b, c) = (3.4445, -4.7750, 2.0315): the odd quintic pushes every singular value of X into [0.68, 1.21] and
-// leaves the singular vectors, so the result is close to U V' of G = U S V'.  [0, 1.2024] is mapped into itself, so
-// |X|_2 <= 1.2024, |A|_2 <= 1.45 and |B|_2 <= 2.81 (B = b A + c A A) from the first step on: fixed powers of two place
-// X, A and B in fp16's range.  Matrices with more rows than columns are worked on as their transpose (m <= n throughout).
+// with (a, b, c) = (3.4445, -4.7750, 2.0315).  Iteration, coefficients and the momentum below are those published as Muon
+// (K. Jordan and others, 2024), the step's factor 0.2 sqrt(max(rows, cols)) is J. Liu and others' (2025).  The odd quintic
+// pushes every singular value of X into [0.68, 1.21] and leaves the singular vectors, so the result is close to U V' of
+// G = U S V'.  [0, 1.2024] is mapped into itself, so |X|_2 <= 1.2024, |A|_2 <= 1.45 and |B|_2 <= 2.81 (B = b A + c A A) from
+// the first step on: fixed powers of two place X, A and B in fp16's range.  Matrices with more rows than columns are worked
+// on as their transpose (m <= n throughout).
 //
 // Number formats.  The products run on fp16 MFMA with fp32 sums.  Rounding X itself is not an option: a step multiplies
 // what lies in the weak directions by a = 3.44, rounding errors included (measured in 64 bits on rank-deficient G: 4e-2 of
 // |O| with X in fp16, 0.3 in bf16).  X is therefore kept as a PAIR of fp16 numbers, X = hi + lo (22 bits, 4 bytes); the
 // term a X uses both, the products read hi alone: their errors pass through B, whose left space is that of the strong
 // directions, and are not multiplied up.  The diagonals of A and B, the largest entries, stay in fp32 vectors beside the
-// fp16 off-diagonals.  Together: 4e-5 ... 1.5e-3 of |O| for every spectrum tried (bf16 operands: up to 1.5e-2).
+// fp16 off-diagonals.  Together, in an emulation of these roundings over nine shapes: 2e-4 ... 1.7e-3 of |O| for Gaussian,
+// decaying and low-rank G, up to 2.8e-3 where all singular values are equal (bf16 operands: up to 1.5e-2).  A bf16 result
+// is off by 1.7e-3 from its own rounding; with these it is 1.9e-3 ... 2.3e-3 on gradients.
 //
-// Every matrix of a call goes through the same launches: one to sum |G|^2 in parts (fp64), one to write X0, three per
-// step (A, B, X; four where A's contraction is cut).  A workgroup finds its matrix in a table of running tile counts (one
-// load per lane and a ballot).  A and B are symmetric: the tiles on and below the diagonal are computed and written twice.
-// A call of small matrices alone takes one workgroup per matrix for all steps (k_orth_small).
+// Every matrix of a call goes through the same launches: one for each 16 entries of the table (orthogonalise alone; the
+// optimizer's table is kept), one to sum |G|^2 in parts (fp64), one to write X0, three per step (A, B, X; four where A's
+// contraction is cut), one more in the optimizer where it clips.  A workgroup finds its matrix in a table of running tile
+// counts (one load per lane and a ballot).  A and B are symmetric: the tiles on and below the diagonal are computed and
+// written twice.  A call of small matrices alone takes one workgroup per matrix for all steps (k_orth_small).
 //
-// Measured, five steps on the GPU (fp32 G, a large library product in fp16 reaches 1107 TFLOP/s, a large copy 4.9 TB/s):
-// 48 matrices of 384-channel blocks 470 us, 2048 x 8192 (bf16 G) 875 us = 640 TFLOP/s of the 558 GFLOP that the symmetric
-// halves need, 96 x 96 30 us.  Bounds: A and B the stream from L2 into LDS (with the products taken out 21 of 25 us
-// remain); X at K = 384 its own reads and writes (hi, lo in; hi, lo out: 8 bytes an element, 5.4 TB/s), at K = 2048 the
-// same stream (66 of 88 us); below about 300 rows the launches, 4 to 6 us each.
+// Measured, five steps, a call among others (fp32 G, a large library product in fp16 reaches 1107 TFLOP/s, a large copy
+// 4.9 TB/s): 48 matrices of 384-channel blocks 445 ... 475 us, 2048 x 8192 (bf16 G) 805 ... 840 us = 680 TFLOP/s of the 558
+// GFLOP that the symmetric halves need, 96 x 96 30 us.  Bounds, from the kernels' own times: A and B the stream from L2 into
+// LDS (2048 x 8192, with the products taken out: 33 of 46 us remain of A, 21 of 24 of B); X at K = 2048 the same stream (66
+// of 88 us); X at K = 384 neither rate: 47.5 us are 3.6 TB/s of its own reads and writes (hi, lo in; hi, lo out: 8 bytes an
+// element; 4.1 TB/s of the measured bytes) and 340 TFLOP/s, with six stages between the two; below about 300 rows the
+// launches, 4 to 10 us each.
 #include "common.h"
 #include <type_traits>
 

@@ -16,7 +16,8 @@ _TYPE = {torch.float32: L.SWG_F32, torch.bfloat16: L.SWG_BF16, torch.float16: L.
 def orthogonalise(g, steps=5, eps=1e-7, out_dtype=torch.bfloat16):
     """Orthogonalised matrices of ``g``: a tensor [rows, cols] or [batch, rows, cols], or a list of such tensors of any
     shapes (one type, one device), which go through the same launches.  float32, bfloat16 or float16 in; bfloat16 or
-    float16 out (the products carry 11 bits).  A zero matrix gives zero.  Not differentiable: a matrix that asks for a
+    float16 out: the products carry 11 bits, which leaves an error of 1e-3 ... 2e-3 of |O| beside the output's rounding (up to
+    3e-3 where all singular values are equal).  A zero matrix gives zero.  Not differentiable: a matrix that asks for a
     gradient in grad mode, one with a forward-mode tangent and a trace are refused.  The work is queued on the current stream and may be recorded into a graph."""
     single = isinstance(g, torch.Tensor)
     mats = [g] if single else list(g)
