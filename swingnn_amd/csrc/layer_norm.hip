@@ -74,7 +74,7 @@ __device__ __forceinline__ double dpp_add(double v) {
   return v + __builtin_bit_cast(double, o);
 }
 template <int LANES>
-__device__ __forceinline__ double group_sum(double v) {
+__device__ __forceinline__ double group_sum64(double v) {
   if constexpr (LANES >= 16) {
     if constexpr (LANES == 64) {
       const uint2 u = __builtin_bit_cast(uint2, v);
@@ -101,11 +101,13 @@ __device__ __forceinline__ double group_sum(double v) {
 // that one barrier a call is enough.
 template <int LANES, class A>
 __device__ __forceinline__ A row_sum(A v, A* red, int& slot) {
+  constexpr int G = LANES < 64 ? LANES : 64;
+  if constexpr (sizeof(A) == 8) v = group_sum64<G>(v);
+  else v = group_sum<G>(v);
   if constexpr (LANES <= 64) {
-    return group_sum<LANES>(v);
+    return v;
   } else {
     constexpr int W = LANES / 64;
-    v = group_sum<64>(v);
     A* r = red + slot * W;
     slot ^= 1;
     if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
