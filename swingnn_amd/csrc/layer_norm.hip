@@ -16,8 +16,8 @@
 // registers; the row groups of a workgroup are joined by shuffles and LDS, the workgroups by k_ln_cols.  The next row's
 // x and dy are loaded before the present row's sums where the registers hold both.
 // Measured (a large copy reaches 4.9 TB/s; kernel times under rocprofv3): forward 516096 x 96 fp32 76 us (5.2 TB/s; part of
-// x stays in the memory-side cache), backward 184320 x 192 fp32 89 us (4.8 TB/s of x, dy, dx), 8192 x 4096 bf16 forward
-// 26 us (5.1 TB/s), backward 53 us (3.8 TB/s, and 34 MB of partial sums), 4097 x 1001 fp16 forward 7, backward 16 + 4 us.
+// x stays in the memory-side cache), backward 184320 x 192 fp32 96 us (4.4 TB/s of x, dy, dx), 8192 x 4096 bf16 forward
+// 25 us (5.4 TB/s), backward 50 us (4.0 TB/s, and 34 MB of partial sums), 4097 x 1001 fp16 forward 6.5, backward 15 + 4 us.
 #include "common.h"
 #include <type_traits>
 
@@ -133,7 +133,7 @@ __device__ __forceinline__ A row_sum(A v, A* red, int& slot) {
 // exact for a mean of 30000 as for one of 0.  A float32 sum leaves a few steps of the mean in every element, which
 // r <= 1 / sqrt(eps) = 316 multiplies (rows of values around 30000.7, a few steps apart: y off by up to 3.3).  Sums of equal
 // values are exact here (24 + 24 bits), and so is s - D hi.  `inv` is 1 / D.  Float32 / 64-bit sums: 516096 x 96 fp32
-// 74.0 / 75.1 us, 184320 x 192 47.0 / 47.9 us, 8192 x 4096 bf16 24.1 / 24.9 us, 4096 x 16384 fp32 111.9 / 117.4 us.
+// 74.0 / 75.1 us, 184320 x 192 47.0 / 47.9 us, 8192 x 4096 bf16 24.1 / 24.9 us, 4096 x 16384 fp32 111.9 / 116.4 us.
 // A chunk of a half type (11 bits at most) is summed in float32 first, which is exact for values within a factor of two.
 template <class T, int N>
 __device__ __forceinline__ double chunk_sum(const float* v, int lo) {  // of the elements from `lo` on
