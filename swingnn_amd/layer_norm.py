@@ -22,7 +22,7 @@ _TYPE = {torch.float32: L.SWG_F32, torch.bfloat16: L.SWG_BF16, torch.float16: L.
 def _rows(t, D):
     """t as [rows, D] with unit stride along D, without a copy where its strides allow it."""
     if D == 1:
-        t = t.resolve_neg()  # the sign flag of z.conj().imag: for wider rows its stride of two has a copy made, which resolves it
+        t = t.resolve_neg()  # the sign flag of z.conj().imag; wider rows of it have a stride of two, and their copy resolves it
     if t.dim() != 2:
         try:
             t = t.view(-1, D)

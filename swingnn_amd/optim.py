@@ -229,9 +229,9 @@ class FusedMuonEMA(FusedAdamEMA):
     layers, and everything else.  Weight decay is decoupled for the matrices and Adam's L2 term for the others.
     Every matrix goes through the same launches, whatever their number: 2 + 3 ns_steps (4 ns_steps where a contraction of
     2048 and more is cut; 4 in all where every matrix is small enough for one workgroup, which no whole network's are), one
-    for the clip and one for the other parameters.  The update is as exact as ``orthogonalise``; where
-    momentum and gradient cancel to rounding its norm counts as at least 2^-17 of theirs.  ``v`` covers the matrices too
-    (one flat layout) and stays zero there."""
+    for the clip and one for the other parameters.  The update is as exact as ``orthogonalise``; where momentum and gradient
+    cancel to rounding its norm counts as at least 2^-17 of theirs.  ``v`` covers the matrices too (one flat layout) and
+    stays zero there."""
 
     def __init__(self, matrices, others=(), lr=1e-4, momentum=0.95, nesterov=True, ns_steps=5, weight_decay=0.0, betas=(0.9, 0.999),
                  eps=1e-8, update_rms=0.2, max_norm=None, ema_betas=(), ema_inv_gamma=1.0, ema_power=1.0):

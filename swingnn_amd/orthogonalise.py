@@ -16,9 +16,10 @@ _TYPE = {torch.float32: L.SWG_F32, torch.bfloat16: L.SWG_BF16, torch.float16: L.
 def orthogonalise(g, steps=5, eps=1e-7, out_dtype=torch.bfloat16):
     """Orthogonalised matrices of ``g``: a tensor [rows, cols] or [batch, rows, cols], or a list of such tensors of any
     shapes (one type, one device), which go through the same launches.  float32, bfloat16 or float16 in; bfloat16 or
-    float16 out: the products carry 11 bits, which leaves an error of 1e-3 ... 2e-3 of |O| beside the output's rounding (up to
-    3e-3 where all singular values are equal).  A zero matrix gives zero.  Not differentiable: a matrix that asks for a
-    gradient in grad mode, one with a forward-mode tangent and a trace are refused.  The work is queued on the current stream and may be recorded into a graph."""
+    float16 out: the products carry 11 bits, which leaves an error of 1e-3 ... 2e-3 of |O| beside the output's rounding (up
+    to 3e-3 where all singular values are equal).  A zero matrix gives zero.  Not differentiable: a matrix that asks for a
+    gradient in grad mode, one with a forward-mode tangent and a trace are refused.  The work is queued on the current
+    stream and may be recorded into a graph."""
     single = isinstance(g, torch.Tensor)
     mats = [g] if single else list(g)
     refuse_transforms("orthogonalise", mats)
@@ -45,7 +46,7 @@ def orthogonalise(g, steps=5, eps=1e-7, out_dtype=torch.bfloat16):
     outs, items, keep = [], (L.SwgOrthItem * len(mats))(), []
     for t, it in zip(mats, items):
         rows, cols = t.shape[-2:]
-        t = t.detach().resolve_neg()  # z.conj().imag holds its sign as a flag, which a column keeps through the strides below
+        t = t.detach().resolve_neg()  # z.conj().imag holds its sign as a flag, which a column keeps through what follows
         # a row of one element has no stride of its own
         if t.numel() and ((cols > 1 and t.stride(-1) != 1) or (rows > 1 and t.stride(-2) < cols)):
             t = t.contiguous()
